@@ -90,6 +90,33 @@ UNTYPED = {
 }
 
 
+# include/graphop_terms.h: the attention layers with learned score terms
+TERMS_BUCKET_FWD, TERMS_BUCKET_BWD, TERMS_DIFF_FWD, TERMS_DIFF_BWD, TERMS_RELATIVE = range(5)
+TERMS_SIGNATURES = {
+    "attention_bucket_forward": [_P] * 3 + [_I64] + [_P] * 5 + [_INT, _DBL] + [_P] * 2 + [_I64] * 3 + [_INT] * 2 + _TAIL,
+    "attention_bucket_backward": [_P] * 3 + [_I64] + [_P] * 4 + [_I64] + [_P] * 5 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 4
+                                 + [_I64] * 3 + [_INT] * 2 + _TAIL,
+    "attention_diff_forward": [_P] * 3 + [_I64] + [_P] * 6 + [_INT, _DBL] + [_P] * 3 + [_I64] * 3 + [_INT] * 2 + _TAIL,
+    "attention_diff_backward": [_P] * 3 + [_I64] + [_P] * 4 + [_I64] + [_P] * 6 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 5
+                               + [_I64] * 3 + [_INT] * 2 + _TAIL,
+}
+TERMS_PLANNED_SIGNATURES = {
+    "attention_bucket_forward_planned": [_PP] + [_P] * 5 + [_INT, _DBL] + [_P] * 2 + [_I64] * 2 + [_INT] * 2 + _TAIL,
+    "attention_bucket_backward_planned": [_PP] * 2 + [_P] * 5 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 4 + [_I64] * 2
+                                         + [_INT] * 2 + _TAIL,
+    "attention_diff_forward_planned": [_PP] + [_P] * 6 + [_INT, _DBL] + [_P] * 3 + [_I64] * 2 + [_INT] * 2 + _TAIL,
+    "attention_diff_backward_planned": [_PP] * 2 + [_P] * 6 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 5 + [_I64] * 2
+                                       + [_INT] * 2 + _TAIL,
+}
+TERMS_UNTYPED = {
+    "graphop_terms_workspace_bytes": ([_INT, _I64, _I64] + [_INT] * 5, _SZ),
+    "graphop_relative_buckets_i32": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64] + _TAIL, _INT),
+    "graphop_relative_buckets_i64": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64] + _TAIL, _INT),
+    "graphop_relative_buckets_planned_i32": ([_PP] + [_P] * 3 + [_INT] * 2 + [_P] * 2, _INT),
+    "graphop_relative_buckets_planned_i64": ([_PP] + [_P] * 3 + [_INT] * 2 + [_P] * 2, _INT),
+}
+
+
 DLPACK_ENTRY_POINTS = ["graphop_dl_" + op for op in (
     "maskedmm_csr_forward", "maskedmm_csr_backward", "node_mul_edge_forward", "node_mul_edge_backward",
     "sparse_softmax_forward", "sparse_softmax_backward", "vector_spmm_forward", "vector_spmm_backward",
@@ -109,29 +136,35 @@ def exported_symbols():
     return names
 
 
+def terms_symbols():
+    """Every symbol include/graphop_terms.h declares."""
+    names = list(TERMS_UNTYPED)
+    for op in TERMS_SIGNATURES:
+        names += ["graphop_%s_%s_%s" % (op, e, i) for e in ELEM_SUFFIXES for i in INDEX_SUFFIXES]
+    for op in TERMS_PLANNED_SIGNATURES:
+        names += ["graphop_%s_%s" % (op, e) for e in ELEM_SUFFIXES]
+    return names
+
+
 _lib = None
 
 
 def bind(handle, strict=True):
-    """Sets argtypes / restype of every entry point of include/graphop_b200.h on a loaded library.
-    strict=False skips symbols the library does not export (a build with fewer element types)."""
-    for name, (args, res) in UNTYPED.items():
-        fn = getattr(handle, name, None) if not strict else getattr(handle, name)
+    """Sets argtypes / restype of every entry point of include/graphop_b200.h and include/graphop_terms.h on a loaded
+    library.  strict=False skips symbols the library does not export (a build with fewer element types)."""
+    def one(name, args, res):
+        fn = getattr(handle, name) if strict else getattr(handle, name, None)
         if fn is not None:
             fn.argtypes, fn.restype = args, res
-    for op, args in SIGNATURES.items():
+    for name, (args, res) in {**UNTYPED, **TERMS_UNTYPED}.items():
+        one(name, args, res)
+    for op, args in {**SIGNATURES, **TERMS_SIGNATURES}.items():
         for e in ELEM_SUFFIXES:
             for i in INDEX_SUFFIXES:
-                name = "graphop_%s_%s_%s" % (op, e, i)
-                fn = getattr(handle, name, None) if not strict else getattr(handle, name)
-                if fn is not None:
-                    fn.argtypes, fn.restype = args, _INT
-    for op, args in PLANNED_SIGNATURES.items():
+                one("graphop_%s_%s_%s" % (op, e, i), args, _INT)
+    for op, args in {**PLANNED_SIGNATURES, **TERMS_PLANNED_SIGNATURES}.items():
         for e in ELEM_SUFFIXES:
-            name = "graphop_%s_%s" % (op, e)
-            fn = getattr(handle, name, None) if not strict else getattr(handle, name)
-            if fn is not None:
-                fn.argtypes, fn.restype = args, _INT
+            one("graphop_%s_%s" % (op, e), args, _INT)
     return handle
 
 

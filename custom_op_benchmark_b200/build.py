@@ -20,7 +20,8 @@ BENCH_LIB = os.path.join(HERE, "libgraphop_b200_bench.so")
 OBJ_DIR = os.path.join(HERE, "build")
 UNITS = ["graphop_capi_f32.cu", "graphop_capi_f64.cu", "graphop_capi_bf16.cu", "graphop_capi_attn_f32.cu",
          "graphop_capi_attn_f64.cu", "graphop_capi_attn_bf16.cu", "graphop_capi_misc.cu", "graphop_capi_static.cu",
-         "graphop_capi_dlpack.cu", "graphop_capi_prep.cu"]
+         "graphop_capi_dlpack.cu", "graphop_capi_prep.cu", "graphop_capi_terms_f32.cu", "graphop_capi_terms_f64.cu",
+         "graphop_capi_terms_bf16.cu", "graphop_capi_terms.cu"]
 # the instrumented twin: what bench.py's workloads call, plus the hooks themselves
 BENCH_UNITS = ["graphop_capi_f32.cu", "graphop_capi_attn_f32.cu", "graphop_capi_attn_bf16.cu", "graphop_capi_misc.cu",
                os.path.join("bench", "graphop_bench.cu")]
@@ -55,7 +56,7 @@ def _build_one_module(name, force):
     from torch.utils import cpp_extension as ce
     out, src = module_path(name), os.path.join(BINDING_DIR, MODULES[name])
     deps = [src, LIB, os.path.join(HERE, "..", "include", "graphop_b200.h"),
-            os.path.join(HERE, "..", "include", "graphop_dlpack.h")]
+            os.path.join(HERE, "..", "include", "graphop_dlpack.h"), os.path.join(HERE, "..", "include", "graphop_terms.h")]
     if not force and not _stale(out, deps):
         return out
     os.makedirs(MODULE_DIR, exist_ok=True)
@@ -81,6 +82,7 @@ def _sources():
         deps += [os.path.join(root, f) for f in files if f.endswith((".cu", ".cuh", ".h"))]
     deps.append(os.path.join(HERE, "..", "include", "graphop_b200.h"))
     deps.append(os.path.join(HERE, "..", "include", "graphop_dlpack.h"))
+    deps.append(os.path.join(HERE, "..", "include", "graphop_terms.h"))
     return deps
 
 

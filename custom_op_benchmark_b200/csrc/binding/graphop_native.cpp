@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "../../../include/graphop_b200.h"
+#include "../../../include/graphop_terms.h"
 
 namespace {
 
@@ -159,6 +160,10 @@ GRAPHOP_OVERLOADS(vector_spmm_forward)
 GRAPHOP_OVERLOADS(vector_spmm_backward)
 GRAPHOP_OVERLOADS(attention_bias_forward)
 GRAPHOP_OVERLOADS(attention_bias_backward)
+GRAPHOP_OVERLOADS(attention_bucket_forward)
+GRAPHOP_OVERLOADS(attention_bucket_backward)
+GRAPHOP_OVERLOADS(attention_diff_forward)
+GRAPHOP_OVERLOADS(attention_diff_backward)
 #undef GRAPHOP_OVERLOADS
 #define GRAPHOP_OVERLOADS(op)                                                                                        \
   template <class... X> int op(float*, X... x) { return graphop_##op##_f32(x...); }                                  \
@@ -166,6 +171,10 @@ GRAPHOP_OVERLOADS(attention_bias_backward)
   template <class... X> int op(uint16_t*, X... x) { return graphop_##op##_bf16(x...); }
 GRAPHOP_OVERLOADS(attention_forward_planned)
 GRAPHOP_OVERLOADS(attention_backward_planned)
+GRAPHOP_OVERLOADS(attention_bucket_forward_planned)
+GRAPHOP_OVERLOADS(attention_bucket_backward_planned)
+GRAPHOP_OVERLOADS(attention_diff_forward_planned)
+GRAPHOP_OVERLOADS(attention_diff_backward_planned)
 #undef GRAPHOP_OVERLOADS
 
 // ------------------------------------------------------------------------------------------
@@ -177,12 +186,12 @@ template <class N, class Save>
 void record(std::initializer_list<Tensor> inputs, Tensor& output, Save&& save) {
   if (!c10::GradMode::is_enabled()) return;
   bool any = false;
-  for (const Tensor& t : inputs) any = any || t.requires_grad();
+  for (const Tensor& t : inputs) any = any || (t.defined() && t.requires_grad());
   if (!any) return;
   std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
   torch::autograd::edge_list edges;
   edges.reserve(inputs.size());
-  for (const Tensor& t : inputs) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  for (const Tensor& t : inputs) edges.push_back(t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge());
   for (auto& e : edges)
     if (!e.function) e = torch::autograd::Edge();
   node->set_next_edges(std::move(edges));
@@ -594,6 +603,250 @@ Result attention_bias(const Tensor& row, const Tensor& indptr, const Tensor& ind
   return o;
 }
 
+// ---- attention with learned score terms: a bias by buckets, differential attention ----------
+// The graph of such a call: plans, or the chunk tables of both orientations (row, indptr, indices; col, indptr_t, eid_t,
+// indices_t, of which only the backward reads the last four).
+struct TermsGraph {
+  GraphPtr rows, cols;
+  Tensor t[7];
+  bool planned() const { return rows != nullptr; }
+  int64_t edges() const { return planned() ? rows->plan.n_edges : t[2].size(0); }
+};
+struct TermsInputs { Tensor q, k, v, lam, bucket, table; };
+struct TermsShape { int elem, H, D, buckets; int64_t n, m; };
+
+void check_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others)
+    if (t->defined() && t->device() != first.device()) fail("expected all tensors of the call on " + first.device().str());
+}
+// graphop.py's checks of the same call, with its texts
+TermsShape check_terms(const TermsInputs& x, bool diff, int64_t edges) {
+  check_input(x.q, "q"); check_input(x.k, "k"); check_input(x.v, "v");
+  if (diff) check_input(x.lam, "lam");
+  TermsShape s;
+  s.elem = elem_of({&x.q, &x.k, &x.v});
+  if (diff) elem_of({&x.q, &x.lam});
+  if (x.table.defined()) elem_of({&x.q, &x.table});
+  check_device(x.q, {&x.k, &x.v, &x.lam});
+  for (const Tensor* t : {&x.q, &x.k, &x.v}) {
+    if (diff && t->dim() != 3) fail("q, k and v must be (n, 2h, d), (n, 2h, d) and (n, h, 2d)");
+    node_shape(*t);
+  }
+  const NodeShape q = node_shape(x.q);
+  s.n = q.n; s.m = x.k.size(0); s.D = q.D; s.H = q.H;
+  if (x.k.sizes().slice(1) != x.q.sizes().slice(1) || x.k.size(0) != x.v.size(0)) fail("q, k and v disagree on their shapes");
+  if (!diff) {
+    if (x.v.sizes().slice(1) != x.q.sizes().slice(1)) fail("q, k and v disagree on their shapes");
+  } else {
+    if (s.H % 2 || x.v.size(1) != s.H / 2 || x.v.size(2) != 2 * s.D) fail("q, k and v must be (n, 2h, d), (n, 2h, d) and (n, h, 2d)");
+    s.H /= 2;
+    if (x.lam.dim() != 1 || x.lam.size(0) != s.H) fail("lam must be (h,)");
+  }
+  s.buckets = 0;
+  if (!x.bucket.defined() && !x.table.defined()) {
+    if (!diff) fail("bucket and table must be given");
+    return s;
+  }
+  if (!x.bucket.defined() || !x.table.defined()) fail(diff ? "bucket and table come together" : "bucket and table must be given");
+  check_input(x.bucket, "bucket"); check_input(x.table, "table");
+  const int64_t columns = diff ? 2 * s.H : s.H;
+  if (x.bucket.scalar_type() != at::kInt || x.bucket.dim() != 1 || x.bucket.size(0) != edges) fail("bucket must be an int32 tensor of (e,)");
+  if (x.table.dim() != 2 || x.table.size(1) != columns || x.table.size(0) < 1) fail("table must be (buckets, " + std::to_string(columns) + ")");
+  check_device(x.q, {&x.bucket, &x.table});
+  s.buckets = (int)std::min<int64_t>(x.table.size(0), std::numeric_limits<int>::max());
+  return s;
+}
+void check_terms_plan(const PlanHandle& plan_r, int64_t n) {
+  if (n < plan_r.graph->plan.n_nodes)
+    fail("q must have a row for each of the plan's " + std::to_string(plan_r.graph->plan.n_nodes) + " nodes");
+}
+void terms_workspace(Call& c, int op, int64_t e, const TermsShape& s, const Tensor& like, int index_bytes) {
+  c.bytes = graphop_terms_workspace_bytes(op, e, std::max(s.n, s.m), s.H, s.D, s.buckets, (int)like.element_size(), index_bytes);
+  c.scratch = at::empty({(int64_t)c.bytes + 256}, like.options().dtype(at::kByte));
+  c.ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(c.scratch.data_ptr()) + 255) / 256 * 256);
+}
+const int32_t* ids(const Tensor& bucket) { return bucket.defined() ? bucket.data_ptr<int32_t>() : nullptr; }
+
+struct TermsBackward : GraphNode {
+  bool diff = false;
+  GraphPtr rows, cols;
+  double scale = 1.0;
+  std::string name() const override {
+    return std::string("GraphAttention") + (diff ? "Diff" : "Bucket") + (rows ? "Planned" : "") + "Backward";
+  }
+  variable_list apply(variable_list&& grads) override {
+    const size_t n_grads = diff ? 5 : 4;   // q, k, v (, lam), table
+    if (!grads[0].defined()) return variable_list(n_grads);
+    const std::vector<Tensor> t = unpack_saved();   // q, k, v, lam, bucket, table, lse, o or parts (, the seven index tensors)
+    const TermsInputs x{t[0], t[1], t[2], t[3], t[4], t[5]};
+    const Tensor &lse = t[6], &o = t[7], g = upstream(grads, "d_o");
+    const bool planned = rows != nullptr;
+    const int64_t e = planned ? rows->plan.n_edges : t[10].size(0);
+    const TermsShape s = check_terms(x, diff, e);
+    elem_of({&x.q, &o, &g});
+    int ib = 4;
+    if (!planned) {
+      const std::vector<Tensor> index(t.begin() + 8, t.begin() + 15);
+      ib = check_columns(index, 3, 7, {"col", "indptr_t", "eid_t", "indices_t"});
+      if (index[5].size(0) != e || index[6].size(0) != e) fail("the transposed CSR must have as many positions as the row CSR");
+    } else {
+      if (s.n < rows->plan.n_nodes || s.m < cols->plan.n_nodes) fail("q and k must have a row for each of the plans' nodes");
+      if (cols->plan.n_edges != e) fail("the plans disagree on the number of edges");
+      if (e && !cols->plan.eid) fail("the transposed CSR's plan must have edge ids");
+    }
+    Call c(x.q);
+    Tensor dq = at::empty_like(x.q.detach()), dk = at::empty_like(x.k.detach()), dv = at::empty_like(x.v.detach()), dl, dt;
+    if (diff) dl = at::empty_like(x.lam.detach());
+    if (s.buckets) dt = at::empty_like(x.table.detach());
+    terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_BWD : GRAPHOP_TERMS_BUCKET_BWD, e, s, x.q, ib);
+    const char* what = diff ? "attention_diff_backward" : "attention_bucket_backward";
+    // f(graph arguments..., then) with `then` the arguments after the graph's
+    const auto typed = [&](auto* y, auto&& call) {
+      using E = std::remove_pointer_t<decltype(y)>;
+      const E *q = ptr<E>(x.q), *k = ptr<E>(x.k), *v = ptr<E>(x.v), *lam = ptr<E>(x.lam), *table = ptr<E>(x.table), *out = ptr<E>(o),
+              *up = ptr<E>(g);
+      return call(q, k, v, lam, ids(x.bucket), table, s.buckets, out, (const void*)lse.data_ptr(), up, scale, ptr<E>(dq), ptr<E>(dk),
+                  ptr<E>(dv), ptr<E>(dl), ptr<E>(dt));
+    };
+    int rc;
+    if (planned) {
+      const graphop_plan_t *pr = &rows->plan, *pt = &cols->plan;
+      rc = by_elem(s.elem, [&](auto* y) {
+        return typed(y, [&](auto q, auto k, auto v, auto lam, auto bucket, auto table, int nb, auto out, auto l, auto up, double sc, auto a,
+                            auto b, auto d, auto gl, auto gt) {
+          return diff ? attention_diff_backward_planned(y, pr, pt, q, k, v, lam, bucket, table, nb, out, l, up, sc, a, b, d, gl, gt, s.n, s.m,
+                                                        s.H, s.D, c.ws, c.bytes, raw(c.stream))
+                      : attention_bucket_backward_planned(y, pr, pt, q, k, v, bucket, table, nb, out, l, up, sc, a, b, d, gt, s.n, s.m, s.H,
+                                                          s.D, c.ws, c.bytes, raw(c.stream));
+        });
+      });
+    } else {
+      rc = by_types(s.elem, ib, [&](auto* y, auto* i) {
+        using I = std::remove_pointer_t<decltype(i)>;
+        const auto in = [&](int at) { return (const I*)ptr<I>(t[8 + at]); };
+        const int64_t chunks = t[8].size(0), chunks_t = t[11].size(0);
+        return typed(y, [&](auto q, auto k, auto v, auto lam, auto bucket, auto table, int nb, auto out, auto l, auto up, double sc, auto a,
+                            auto b, auto d, auto gl, auto gt) {
+          return diff ? attention_diff_backward(y, i, owners<I>(t[8], t[9]), in(1), in(2), chunks, owners<I>(t[11], t[12]), in(4), in(5), in(6),
+                                                chunks_t, q, k, v, lam, bucket, table, nb, out, l, up, sc, a, b, d, gl, gt, e, s.n, s.m, s.H,
+                                                s.D, c.ws, c.bytes, raw(c.stream))
+                      : attention_bucket_backward(y, i, owners<I>(t[8], t[9]), in(1), in(2), chunks, owners<I>(t[11], t[12]), in(4), in(5),
+                                                  in(6), chunks_t, q, k, v, bucket, table, nb, out, l, up, sc, a, b, d, gt, e, s.n, s.m, s.H,
+                                                  s.D, c.ws, c.bytes, raw(c.stream));
+        });
+      });
+    }
+    check_status(rc, planned ? (diff ? "attention_diff_backward_planned" : "attention_bucket_backward_planned") : what);
+    if (diff) return {dq, dk, dv, dl, dt};
+    return {dq, dk, dv, dt};
+  }
+};
+
+Tensor terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, double scale) {
+  const int64_t e = graph.edges();
+  int ib = 4;
+  if (!graph.planned()) {
+    check_input(graph.t[0], "row"); check_input(graph.t[1], "indptr"); check_input(graph.t[2], "indices");
+    ib = index_bytes_of({&graph.t[0], &graph.t[1], &graph.t[2]});
+    check_chunks(graph.t[0], graph.t[1]);
+  }
+  const TermsShape s = check_terms(x, diff, e);
+  Call c(x.q);
+  bool grads = false;
+  if (c10::GradMode::is_enabled())
+    for (const Tensor* t : {&x.q, &x.k, &x.v, &x.lam, &x.table}) grads = grads || (t->defined() && t->requires_grad());
+  Tensor o = at::empty(x.v.dim() == 3 ? std::vector<int64_t>{s.n, x.v.size(1), x.v.size(2)} : std::vector<int64_t>{s.n, x.v.size(1)},
+                       x.q.options());
+  const int64_t maps = diff ? 2 * s.H : s.H;
+  Tensor lse = at::empty({s.n, maps}, x.q.options().dtype(s.elem == 1 ? at::kDouble : at::kFloat)), parts;
+  if (diff && grads) parts = at::empty({s.n, s.H, 2, 2 * s.D}, x.q.options());
+  terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_FWD : GRAPHOP_TERMS_BUCKET_FWD, e, s, x.q, ib);
+  const auto typed = [&](auto* y, auto&& call) {
+    using E = std::remove_pointer_t<decltype(y)>;
+    const E *q = ptr<E>(x.q), *k = ptr<E>(x.k), *v = ptr<E>(x.v), *lam = ptr<E>(x.lam), *table = ptr<E>(x.table);
+    return call(q, k, v, lam, ids(x.bucket), table, s.buckets, scale, ptr<E>(o), ptr<E>(parts), (void*)lse.data_ptr());
+  };
+  int rc;
+  if (graph.planned()) {
+    const graphop_plan_t* p = &graph.rows->plan;
+    rc = by_elem(s.elem, [&](auto* y) {
+      return typed(y, [&](auto q, auto k, auto v, auto lam, auto bucket, auto table, int nb, double sc, auto out, auto each, void* l) {
+        return diff ? attention_diff_forward_planned(y, p, q, k, v, lam, bucket, table, nb, sc, out, each, l, s.n, s.m, s.H, s.D, c.ws, c.bytes,
+                                                     raw(c.stream))
+                    : attention_bucket_forward_planned(y, p, q, k, v, bucket, table, nb, sc, out, l, s.n, s.m, s.H, s.D, c.ws, c.bytes,
+                                                       raw(c.stream));
+      });
+    });
+  } else {
+    rc = by_types(s.elem, ib, [&](auto* y, auto* i) {
+      using I = std::remove_pointer_t<decltype(i)>;
+      const I *row = owners<I>(graph.t[0], graph.t[1]), *indptr = ptr<I>(graph.t[1]), *indices = ptr<I>(graph.t[2]);
+      const int64_t chunks = graph.t[0].size(0);
+      return typed(y, [&](auto q, auto k, auto v, auto lam, auto bucket, auto table, int nb, double sc, auto out, auto each, void* l) {
+        return diff ? attention_diff_forward(y, i, row, indptr, indices, chunks, q, k, v, lam, bucket, table, nb, sc, out, each, l, e, s.n, s.m,
+                                             s.H, s.D, c.ws, c.bytes, raw(c.stream))
+                    : attention_bucket_forward(y, i, row, indptr, indices, chunks, q, k, v, bucket, table, nb, sc, out, l, e, s.n, s.m, s.H, s.D,
+                                               c.ws, c.bytes, raw(c.stream));
+      });
+    });
+  }
+  check_status(rc, diff ? (graph.planned() ? "attention_diff_forward_planned" : "attention_diff_forward")
+                        : (graph.planned() ? "attention_bucket_forward_planned" : "attention_bucket_forward"));
+  const auto keep = [&](TermsBackward& n) {
+    n.diff = diff;
+    n.rows = graph.rows;
+    n.cols = graph.cols;
+    n.scale = scale;
+    n.save_all({x.q, x.k, x.v, x.lam, x.bucket, x.table, lse});
+    if (diff) n.save(parts);
+    else n.save(o, true);
+    if (!graph.planned())
+      for (const Tensor& t : graph.t) n.save(t);
+  };
+  if (grads) {
+    if (diff) record<TermsBackward>({x.q, x.k, x.v, x.lam, x.table}, o, keep);
+    else record<TermsBackward>({x.q, x.k, x.v, x.table}, o, keep);
+  }
+  return o;
+}
+
+Result terms_on_tables(std::initializer_list<Tensor> index, const TermsInputs& x, bool diff, double scale) {
+  TermsGraph graph;
+  std::copy(index.begin(), index.end(), graph.t);
+  for (const Tensor& t : graph.t)
+    if (left_to_python({&t})) return c10::nullopt;
+  if (left_to_python({&x.q, &x.k, &x.v, &x.lam, &x.bucket, &x.table})) return c10::nullopt;
+  return terms_forward(graph, x, diff, scale);
+}
+Result terms_on_plans(const PlanHandle& plan_r, const PlanHandle& plan_t, const TermsInputs& x, bool diff, double scale) {
+  if (left_to_python({&x.q, &x.k, &x.v, &x.lam, &x.bucket, &x.table})) return c10::nullopt;
+  check_terms_plan(plan_r, x.q.defined() && x.q.dim() ? x.q.size(0) : 0);
+  TermsGraph graph;
+  graph.rows = plan_r.graph;
+  graph.cols = plan_t.graph;
+  return terms_forward(graph, x, diff, scale);
+}
+Result attention_bucket(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Later& col, const Later& indptr_t,
+                        const Later& eid_t, const Later& indices_t, const Tensor& q, const Tensor& k, const Tensor& v, const Later& bucket,
+                        const Later& table, double scale) {
+  return terms_on_tables({row, indptr, indices, given(col), given(indptr_t), given(eid_t), given(indices_t)},
+                         {q, k, v, Tensor(), given(bucket), given(table)}, false, scale);
+}
+Result attention_diff(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Later& col, const Later& indptr_t,
+                      const Later& eid_t, const Later& indices_t, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam,
+                      double scale, const Later& bucket, const Later& table) {
+  return terms_on_tables({row, indptr, indices, given(col), given(indptr_t), given(eid_t), given(indices_t)},
+                         {q, k, v, lam, given(bucket), given(table)}, true, scale);
+}
+Result attention_bucket_planned_(const PlanHandle& plan_r, const PlanHandle& plan_t, const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const Later& bucket, const Later& table, double scale) {
+  return terms_on_plans(plan_r, plan_t, {q, k, v, Tensor(), given(bucket), given(table)}, false, scale);
+}
+Result attention_diff_planned_(const PlanHandle& plan_r, const PlanHandle& plan_t, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& lam, double scale, const Later& bucket, const Later& table) {
+  return terms_on_plans(plan_r, plan_t, {q, k, v, lam, given(bucket), given(table)}, true, scale);
+}
+
 // ---- graph preparation: graphop.py's functions of the same names ---------------------------
 Tensor scratch_of(size_t bytes, const Tensor& like, void** base) {
   Tensor t = at::empty({(int64_t)bytes + 256}, like.options().dtype(at::kByte));
@@ -672,6 +925,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("vector_spmm", &vector_spmm, free_gil());
   m.def("attention_planned", &attention_planned, free_gil());
   m.def("attention_bias", &attention_bias, free_gil());
+  m.def("attention_bucket", &attention_bucket, free_gil());
+  m.def("attention_bucket_planned", &attention_bucket_planned_, free_gil());
+  m.def("attention_diff", &attention_diff, free_gil());
+  m.def("attention_diff_planned", &attention_diff_planned_, free_gil());
   m.def("partition_csr", &partition_csr, free_gil());
   m.def("transpose_csr", &transpose_csr, free_gil());
   m.def("plan_build", &plan_build, free_gil());

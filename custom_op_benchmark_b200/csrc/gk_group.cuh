@@ -242,6 +242,9 @@ template <class GEO, int kRows, int kScalar, int kState, int kNode, int kNodeSca
 struct Shape {
   static constexpr bool kSums = false;
   static constexpr bool kOptional = false;   // may be one of two walkers launched for the same sums
+  static constexpr bool kComputed = false;   // the table holds values made of what scalar_of finds, not its bytes
+  static constexpr bool kMasks = false;      // a position may take no part, by its edge id
+  struct Raw {};
   static constexpr int kWarps = 1;
   static constexpr int kStepBytes = kRows * GEO::kRow;
   static constexpr int kNodeScalarAt = kNode * GEO::kRow;                  // from the node's room
@@ -313,6 +316,8 @@ __device__ __forceinline__ bool cut_inside(const WalkArgs& a, unsigned j, int r)
 //   setup(st, gl, hb)
 //   stage(st, slot, id, edge, live)               copy the rows of (other endpoint, edge) into the ring
 //   scalar_of(h, id, edge)                        where the edge's scalars of head h are
+//   raw_scalar(h, edge, live), put_scalar(at, Raw)   kComputed: what is fetched of them, and what goes into the table
+//   takes_part(edge)                              kMasks: else the position's rows are zeros and its scalars not live
 //   fold<N>(st, slot, tab, active, pos, edge)     fold N = 1 or 2 positions per group (called by the whole warp); tab: the
 //                                                 table's entry of the first position and this lane's head
 //   stage_node(st, buf, lane, node)               copy what begin(node) will read into the node buffer
@@ -365,6 +370,8 @@ group_walk_kernel(const __grid_constant__ Op op, const __grid_constant__ WalkArg
     e = Op::kUsesEid ? (in ? (a.eid ? __ldg(a.eid + j0 + i) : (int)(j0 + i)) : 0) : 0;
     o = Op::kUsesOther ? (in ? __ldg(a.other + j0 + i) : 0) : 0;
     if (r < 0) { o = -1; e = 0; }
+    if constexpr (Op::kMasks)
+      if (r >= 0 && !op.takes_part(e)) o = -1;
   };
   // bit of every lane whose position (of block b) starts another row than the position before it, or another piece of its row
   auto starts_of = [&](int b, int r, int before_block) {
@@ -410,6 +417,7 @@ group_walk_kernel(const __grid_constant__ Op op, const __grid_constant__ WalkArg
   constexpr int SC = Op::kScalarBytes, TB = Op::kTable, ENTRY = Op::kHeads * SC;
   const unsigned table = ring - lane * Op::SB + 2 * ITER;
   uint16_t held[SC == 2 ? Op::kHeads : 1];
+  [[maybe_unused]] typename Op::Raw raw[Op::kComputed ? Op::kHeads : 1];
   auto fetch_scalars = [&](unsigned tab, int o, int e) {
     if constexpr (SC > 0) {
       const int per = op.block_heads(), pieces = op.parts * op.H - hb * per;   // heads in this block
@@ -417,6 +425,7 @@ group_walk_kernel(const __grid_constant__ Op op, const __grid_constant__ WalkArg
       for (int k = 0; k < Op::kHeads; ++k) {
         const bool live = o >= 0 && k < per && k < pieces;
         const int ph = live ? hb * per + k : 0;
+        if constexpr (Op::kComputed) { raw[k] = op.raw_scalar(ph, e, live); continue; }
         const void* src = op.scalar_of(op.parts == 1 ? ph : ph / op.parts, live ? o : 0, live ? e : 0);
         if constexpr (SC == 2) held[k] = live ? __ldg(reinterpret_cast<const uint16_t*>(src)) : (uint16_t)0;
         else cp_async_slot<SC>(tab + lane * ENTRY + k * SC, src, live);
@@ -424,7 +433,10 @@ group_walk_kernel(const __grid_constant__ Op op, const __grid_constant__ WalkArg
     }
   };
   auto publish_scalars = [&](unsigned tab) {
-    if constexpr (SC == 2) {
+    if constexpr (Op::kComputed) {
+#pragma unroll
+      for (int k = 0; k < Op::kHeads; ++k) op.put_scalar(tab + lane * ENTRY + k * SC, raw[k]);
+    } else if constexpr (SC == 2) {
 #pragma unroll
       for (int k = 0; k < Op::kHeads; ++k)
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(tab + lane * ENTRY + k * SC), "h"(held[k]) : "memory");

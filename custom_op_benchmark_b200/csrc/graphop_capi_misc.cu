@@ -6,40 +6,6 @@
 namespace gk {
 namespace {
 
-// Scratch of one row-producing pass: per level 2 slots per tile, each `stride_bytes`, plus the
-// next level's row stream.
-size_t levels_bytes(long long len0, int tile0, size_t stride_bytes) {
-  const Levels lv = make_levels(len0, tile0);
-  size_t total = 0;
-  for (int k = 0; k + 1 < lv.n; ++k) {
-    total += align_up((size_t)(2 * lv.ntiles[k]) * stride_bytes);
-    total += align_up((size_t)(2 * lv.ntiles[k]) * 4);
-  }
-  return total;
-}
-
-// Carry levels of one pass of the gathering walker over (H, D) rows, `accs` accumulator rows and `stats` more words per
-// lane each, for whatever slot width the operands' alignment allows; the register-fetch walker's when none fits.
-size_t walk_bytes(long long E, long long n_nodes, int H, int D, int elem, bool split, int accs, int stats) {
-  const size_t acc = elem == 8 ? 8 : 4;
-  const int tile = pick_tile(E);
-  size_t most = split ? levels_bytes(E, tile, (size_t)H * D * acc) : 0;
-  for (int align = 16; align >= 4; align >>= 1) {
-    for (const GeoPick& p : {pick_geo(H, D, elem, align, split), pick_sum_geo(H, D, elem, align)}) {
-      if (!p.SB) continue;
-      const size_t b = carry_bytes(tile_bound(E, n_nodes), p.nhb, (long long)accs * p.accs(elem) + stats * p.G, acc);
-      most = b > most ? b : most;
-    }
-  }
-  return most;
-}
-
-size_t graph_bytes(long long E, long long n_nodes, int index_bytes) {
-  size_t b = align_up(sizeof(PlanHeader)) + align_up((size_t)E * 4) + align_up((size_t)(tile_bound(E, n_nodes) + 1) * 4);
-  if (index_bytes == 8) b += 2 * align_up((size_t)E * 4);
-  return b;
-}
-
 template <typename I>
 __global__ void check_graph_kernel(const I* __restrict__ row, const I* __restrict__ indptr, const I* __restrict__ eid,
                                    const I* __restrict__ indices, long long C, long long E, long long n_nodes,

@@ -14,6 +14,7 @@ and float64; ``dy`` is made contiguous instead of being read unchecked
 (graphop.cpp:120-130, 148-153); the source and destination node counts may differ.
 """
 import collections
+import functools
 
 import torch as th
 
@@ -26,7 +27,10 @@ __all__ = [
     "GraphPlan", "maskedmm_csr_forward_planned", "maskedmm_csr_backward_planned", "vector_spmm_forward_planned",
     "vector_spmm_backward_planned", "sparse_softmax_forward_planned", "sparse_softmax_backward_planned",
     "node_mul_edge_forward_planned", "node_mul_edge_backward_planned", "attention_forward_planned",
-    "attention_backward_planned",
+    "attention_backward_planned", "relative_buckets", "relative_buckets_planned", "bucket_limits",
+    "attention_bucket_forward", "attention_bucket_backward", "attention_bucket_forward_planned",
+    "attention_bucket_backward_planned", "attention_diff_forward", "attention_diff_backward",
+    "attention_diff_forward_planned", "attention_diff_backward_planned",
 ]
 
 _ELEM = {th.float32: ("f32", 4), th.float64: ("f64", 8), th.bfloat16: ("bf16", 2)}
@@ -692,3 +696,314 @@ def attention_backward_planned(plan_r, plan_t, q, k, v, o, lse, d_o, scale):
                       [_p(q), _p(k), _p(v), _p(o), _p(lse), _p(d_o), float(scale), _p(dq), _p(dk), _p(dv), q.size(0),
                        k.size(0), h, d])
     return [dq, dk, dv]
+
+
+# ------------------------------------------------------------------------------------------
+# attention with learned score terms (additions): a bias by buckets, differential attention
+# ------------------------------------------------------------------------------------------
+def bucket_limits(num_buckets, max_distance):
+    """The distances at which the buckets of one direction begin, but for the first: bucket b holds the distances that
+    at least b of them do not exceed.  The first half of the buckets hold one distance each; the others share what lies
+    between there and ``max_distance`` evenly over its logarithm, and the last one also holds everything farther:
+    bucket(x) = half + floor((num_buckets - half) * ln(x / half) / ln(max_distance / half)).  In whole numbers: a limit is
+    the smallest x with x^m * half^t >= max_distance^t * half^m, m = num_buckets - half, t = bucket - half."""
+    num_buckets, max_distance = int(num_buckets), int(max_distance)
+    half = num_buckets // 2
+    if num_buckets < 2 or max_distance <= half:
+        raise ValueError("relative positions need two buckets or more a direction, and a max_distance beyond the exact ones")
+    m, found = num_buckets - half, list(range(1, half + 1))
+    for t in range(1, m):
+        want = max_distance ** t * half ** m
+        x = max(half, int(half * (max_distance / half) ** (t / m)) - 1)
+        while x > half and x ** m * half ** t >= want:
+            x -= 1
+        while x ** m * half ** t < want:
+            x += 1
+        found.append(x)
+    return found
+
+
+def _limits(num_buckets, max_distance, bidirectional):
+    import ctypes
+    if bidirectional and num_buckets % 2:
+        raise ValueError("num_buckets must be even for both directions")
+    at = _limits_of(int(num_buckets) // 2 if bidirectional else int(num_buckets), int(max_distance))
+    return (ctypes.c_int64 * len(at))(*at), len(at)
+
+
+@functools.lru_cache(maxsize=64)
+def _limits_of(num_buckets, max_distance):
+    return tuple(bucket_limits(num_buckets, max_distance))
+
+
+def _positions(dst_pos, src_pos, n_dst, n_src, dtype, device):
+    """Both ends' positions, checked; None: the nodes' own numbers."""
+    for t, n, name in ((dst_pos, n_dst, "dst_pos"), (src_pos, n_src, "src_pos")):
+        if t is None:
+            continue
+        _check_input(t, name)
+        if t.dim() != 1 or t.dtype not in _INDEX or (dtype is not None and t.dtype != dtype):
+            raise RuntimeError("%s must be a one-dimensional tensor of the call's index type" % name)
+        if t.device != device:
+            raise RuntimeError("%s must be on the graph's device" % name)
+        if n is not None and t.numel() < n:
+            raise RuntimeError("%s must hold a position for every node" % name)
+        dtype = t.dtype
+    return dtype
+
+
+def relative_buckets(row, indptr, indices, num_buckets, max_distance, bidirectional=True, dst_pos=None, src_pos=None):
+    """The bucket (int32, by row-CSR position) of every edge's relative position src_pos[indices] - dst_pos[row].
+
+    ``bidirectional``: half of the buckets are for positions ahead (a positive difference), the others for the rest;
+    without it all are for positions behind, and those ahead share bucket 0.  Within a direction the distances are
+    shared out as ``bucket_limits`` says.  ``dst_pos`` and ``src_pos`` (index type) default to the node ids; every
+    node that an edge names needs a position."""
+    _check_all(row=row, indptr=indptr, indices=indices)
+    index = _index(row, indptr, indices)
+    e, c = indices.size(0), _chunks(row, indptr)
+    _positions(dst_pos, src_pos, None, None, indices.dtype, indices.device)
+    limits, n = _limits(num_buckets, max_distance, bidirectional)
+    out = th.empty(e, dtype=th.int32, device=indices.device)
+    lib = _capi.lib()
+    with th.cuda.device(out.device):
+        _ws, base, need = _scratch(lib.graphop_terms_workspace_bytes(_capi.TERMS_RELATIVE, e, 0, 1, 1, 0, 4, index[1]),
+                                   out.device)
+        _check(getattr(lib, "graphop_relative_buckets_" + index[0])(
+            _owners(row, indptr), _p(indptr), _p(indices), c, _p(dst_pos), _p(src_pos), limits, n, int(bool(bidirectional)), _p(out), e, base,
+            need, th.cuda.current_stream(out.device).cuda_stream), "relative_buckets")
+    return out
+
+
+def relative_buckets_planned(plan, num_buckets, max_distance, bidirectional=True, dst_pos=None, src_pos=None):
+    """relative_buckets on a plan of the row CSR; the positions are int32 or int64, both the same."""
+    dtype = _positions(dst_pos, src_pos, plan.n_nodes, None, None, plan.device)
+    limits, n = _limits(num_buckets, max_distance, bidirectional)
+    out = th.empty(plan.n_edges, dtype=th.int32, device=plan.device)
+    suffix = "i64" if dtype == th.int64 else "i32"
+    with th.cuda.device(out.device):
+        _check(getattr(_capi.lib(), "graphop_relative_buckets_planned_" + suffix)(
+            plan.ref(), _p(dst_pos), _p(src_pos), limits, n, int(bool(bidirectional)), _p(out),
+            th.cuda.current_stream(out.device).cuda_stream), "relative_buckets_planned")
+    return out
+
+
+def _terms_shape(q, k, v, diff):
+    """(h, d): heads of d features, or pairs of maps of d features each."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 3 and (diff or t.dim() != 2):
+            raise RuntimeError("%s must be (n, 2h, d), (n, 2h, d) and (n, h, 2d)" % "q, k and v" if diff else
+                               "node tensors must be (n, d) or (n, h, d)")
+    h, d = _heads(q, True)
+    if k.shape[1:] != q.shape[1:] or k.size(0) != v.size(0):
+        raise RuntimeError("q, k and v disagree on their shapes")
+    if not diff:
+        if v.shape[1:] != q.shape[1:]:
+            raise RuntimeError("q, k and v disagree on their shapes")
+        return h, d
+    if h % 2 or v.size(1) != h // 2 or v.size(2) != 2 * d:
+        raise RuntimeError("q, k and v must be (n, 2h, d), (n, 2h, d) and (n, h, 2d)")
+    return h // 2, d
+
+
+def _terms_bias(bucket, table, columns, n_edges, device):
+    """The number of buckets, 0 without a bias."""
+    if bucket is None and table is None:
+        return 0
+    if bucket is None or table is None:
+        raise RuntimeError("bucket and table come together")
+    _check_all(bucket=bucket, table=table)
+    if bucket.dtype != th.int32 or bucket.dim() != 1 or bucket.size(0) != n_edges:
+        raise RuntimeError("bucket must be an int32 tensor of (e,)")
+    if table.dim() != 2 or table.size(1) != columns or table.size(0) < 1:
+        raise RuntimeError("table must be (buckets, %d)" % columns)
+    if bucket.device != device or table.device != device:
+        raise RuntimeError("expected all tensors of the call on %s" % device)
+    return table.size(0)
+
+
+def _terms_lam(lam, h):
+    _check_input(lam, "lam")
+    if lam.dim() != 1 or lam.size(0) != h:
+        raise RuntimeError("lam must be (h,)")
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t.device != first.device:
+            raise RuntimeError("expected all tensors of the call on %s" % first.device)
+
+
+def _terms_call(name, graph, elem, op_id, n_edges, n_nodes, h, d, buckets, device, args):
+    """One call of include/graphop_terms.h.  graph: (index suffix, bytes, arguments) of a chunk table, or plans."""
+    lib = _capi.lib()
+    planned = graph[0] is None
+    with th.cuda.device(device):
+        need = lib.graphop_terms_workspace_bytes(op_id, n_edges, n_nodes, h, d, buckets, elem[1], graph[1])
+        _ws, base, need = _scratch(need, device)
+        fn = getattr(lib, "graphop_%s_planned_%s" % (name, elem[0]) if planned else "graphop_%s_%s_%s" % (name, elem[0], graph[0]))
+        _check(fn(*graph[2], *args, base, need, th.cuda.current_stream(device).cuda_stream), name + ("_planned" if planned else ""))
+
+
+def _owners(row, indptr):
+    # a table without chunks has no memory, and the entry points refuse a null pointer: nothing is read through this one
+    return _p(row) if row.numel() else _p(indptr)
+
+
+def _rows_graph(row, indptr, indices):
+    _check_all(row=row, indptr=indptr, indices=indices)
+    index = _index(row, indptr, indices)
+    return (index[0], index[1], [_owners(row, indptr), _p(indptr), _p(indices), _chunks(row, indptr)]), indices.size(0)
+
+
+def _both_graphs(row, indptr, indices, col, indptr_t, eid_t, indices_t):
+    _check_all(row=row, indptr=indptr, indices=indices, col=col, indptr_t=indptr_t, eid_t=eid_t, indices_t=indices_t)
+    index = _index(row, indptr, indices, col, indptr_t, eid_t, indices_t)
+    e = indices.size(0)
+    if eid_t.size(0) != e or indices_t.size(0) != e:
+        raise RuntimeError("the transposed CSR must have as many positions as the row CSR")
+    return (index[0], index[1], [_owners(row, indptr), _p(indptr), _p(indices), _chunks(row, indptr), _owners(col, indptr_t),
+                                 _p(indptr_t), _p(eid_t), _p(indices_t), _chunks(col, indptr_t)]), e
+
+
+def _plan_rows(plan, n_dst):
+    if n_dst < plan.n_nodes:
+        raise RuntimeError("q must have a row for each of the plan's %d nodes" % plan.n_nodes)
+    return (None, 4, [plan.ref()]), plan.n_edges
+
+
+def _plan_both(plan_r, plan_t, n_dst, n_src):
+    if n_dst < plan_r.n_nodes or n_src < plan_t.n_nodes:
+        raise RuntimeError("q and k must have a row for each of the plans' nodes")
+    if plan_t.n_edges != plan_r.n_edges:
+        raise RuntimeError("the plans disagree on the number of edges")
+    if plan_r.n_edges and not plan_t.c.eid:
+        raise RuntimeError("the transposed CSR's plan must have edge ids")
+    return (None, 4, [plan_r.ref(), plan_t.ref()]), plan_r.n_edges
+
+
+def _bucket_forward(graph, e, q, k, v, bucket, table, scale):
+    if bucket is None or table is None:
+        raise RuntimeError("bucket and table must be given")
+    _check_all(q=q, k=k, v=v)
+    elem = _elem(q, k, v, table)
+    _same_device(q, k, v)
+    h, d = _terms_shape(q, k, v, False)
+    nb = _terms_bias(bucket, table, h, e, q.device)
+    o = th.empty_like(q)
+    lse = th.empty((q.size(0), h), dtype=_lse_dtype(q), device=q.device)
+    _terms_call("attention_bucket_forward", graph, elem, _capi.TERMS_BUCKET_FWD, e, max(q.size(0), k.size(0)), h, d, nb, q.device,
+                [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, float(scale), _p(o), _p(lse)] + ([] if graph[0] is None else [e])
+                + [q.size(0), k.size(0), h, d])
+    return o, lse
+
+
+def _bucket_backward(graph, e, q, k, v, bucket, table, o, lse, d_o, scale):
+    d_o = d_o.contiguous()
+    _check_all(q=q, k=k, v=v, o=o, lse=lse, d_o=d_o)
+    elem = _elem(q, k, v, table, o, d_o)
+    _same_device(q, k, v, o, lse, d_o)
+    h, d = _terms_shape(q, k, v, False)
+    nb = _terms_bias(bucket, table, h, e, q.device)
+    if o.shape != q.shape or d_o.shape != q.shape or lse.numel() != q.size(0) * h or lse.dtype != _lse_dtype(q):
+        raise RuntimeError("o, lse and d_o must have the forward's shapes and types")
+    out = [th.empty_like(t) for t in (q, k, v, table)]
+    _terms_call("attention_bucket_backward", graph, elem, _capi.TERMS_BUCKET_BWD, e, max(q.size(0), k.size(0)), h, d, nb, q.device,
+                [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, _p(o), _p(lse), _p(d_o), float(scale)] + [_p(t) for t in out]
+                + ([] if graph[0] is None else [e]) + [q.size(0), k.size(0), h, d])
+    return out
+
+
+def attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale):
+    """(o, lse): attention_forward with a learned bias by buckets in the scores, scale * q[n].k[indices[j]] +
+    table[bucket[j], h] for position j of the row CSR.  ``bucket`` (e,) int32 (``relative_buckets`` makes them of positions; an
+    edge type or a hop distance serves as well), ``table`` (buckets, h) of the node tensors' type.
+
+    A position takes no part where its bucket is outside 0 .. buckets - 1 (-1 marks padding) or its entry of the table is at
+    most -1e38 (-inf, a type's lowest value), whatever its rows hold.  A node of which nothing takes part has o = 0,
+    lse = -inf.  One destination per sequence and its cached rows as sources, in any order, make a decoding step."""
+    graph, e = _rows_graph(row, indptr, indices)
+    return _bucket_forward(graph, e, q, k, v, bucket, table, scale)
+
+
+def attention_bucket_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, q, k, v, bucket, table, o, lse, d_o, scale):
+    """[dq, dk, dv, d_table] of attention_bucket_forward.  eid_t: for every position of the transposed CSR the position of
+    the same edge in the row CSR."""
+    graph, e = _both_graphs(row, indptr, indices, col, indptr_t, eid_t, indices_t)
+    return _bucket_backward(graph, e, q, k, v, bucket, table, o, lse, d_o, scale)
+
+
+def attention_bucket_forward_planned(plan, q, k, v, bucket, table, scale):
+    """attention_bucket_forward on a plan of the row CSR."""
+    graph, e = _plan_rows(plan, q.size(0))
+    return _bucket_forward(graph, e, q, k, v, bucket, table, scale)
+
+
+def attention_bucket_backward_planned(plan_r, plan_t, q, k, v, bucket, table, o, lse, d_o, scale):
+    """attention_bucket_backward on plans of both orientations (plan_t with the transposed CSR's edge ids)."""
+    graph, e = _plan_both(plan_r, plan_t, q.size(0), k.size(0))
+    return _bucket_backward(graph, e, q, k, v, bucket, table, o, lse, d_o, scale)
+
+
+def _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts):
+    _check_all(q=q, k=k, v=v, lam=lam)
+    elem = _elem(q, k, v, lam, *([] if table is None else [table]))
+    _same_device(q, k, v, lam)
+    h, d = _terms_shape(q, k, v, True)
+    _terms_lam(lam, h)
+    nb = _terms_bias(bucket, table, 2 * h, e, q.device)
+    n = q.size(0)
+    o = th.empty((n, h, 2 * d), dtype=q.dtype, device=q.device)
+    parts = th.empty((n, h, 2, 2 * d), dtype=q.dtype, device=q.device) if keep_parts else None
+    lse = th.empty((n, 2 * h), dtype=_lse_dtype(q), device=q.device)
+    _terms_call("attention_diff_forward", graph, elem, _capi.TERMS_DIFF_FWD, e, max(n, k.size(0)), h, d, nb, q.device,
+                [_p(q), _p(k), _p(v), _p(lam), _p(bucket), _p(table), nb, float(scale), _p(o), _p(parts), _p(lse)]
+                + ([] if graph[0] is None else [e]) + [n, k.size(0), h, d])
+    return o, lse, parts
+
+
+def _diff_backward(graph, e, q, k, v, lam, parts, lse, d_o, scale, bucket, table):
+    d_o = d_o.contiguous()
+    _check_all(q=q, k=k, v=v, lam=lam, parts=parts, lse=lse, d_o=d_o)
+    elem = _elem(q, k, v, lam, parts, d_o, *([] if table is None else [table]))
+    _same_device(q, k, v, lam, parts, lse, d_o)
+    h, d = _terms_shape(q, k, v, True)
+    _terms_lam(lam, h)
+    nb = _terms_bias(bucket, table, 2 * h, e, q.device)
+    n = q.size(0)
+    if parts.shape != (n, h, 2, 2 * d) or d_o.shape != (n, h, 2 * d) or lse.shape != (n, 2 * h) or lse.dtype != _lse_dtype(q):
+        raise RuntimeError("parts, lse and d_o must have the forward's shapes and types")
+    out = [th.empty_like(t) for t in (q, k, v, lam)] + ([th.empty_like(table)] if nb else [])
+    _terms_call("attention_diff_backward", graph, elem, _capi.TERMS_DIFF_BWD, e, max(n, k.size(0)), h, d, nb, q.device,
+                [_p(q), _p(k), _p(v), _p(lam), _p(bucket), _p(table), nb, _p(parts), _p(lse), _p(d_o), float(scale)]
+                + [_p(t) for t in out] + ([] if nb else [None]) + ([] if graph[0] is None else [e]) + [n, k.size(0), h, d])
+    return out
+
+
+def attention_diff_forward(row, indptr, indices, q, k, v, lam, scale, bucket=None, table=None, keep_parts=True):
+    """(o, lse, parts): differential attention, o = o1 - lam[h] * o2 with o1 and o2 the softmax sums of v under two maps of
+    scores.  ``q`` (n, 2h, d) and ``k`` (m, 2h, d): heads 2i and 2i + 1 are the maps of head i of ``v`` (m, h, 2d);
+    ``lam`` (h,), of the same type; o (n, h, 2d), lse (n, 2h).  ``parts`` (n, h, 2, 2d), o1 and o2, is what the backward
+    reads (None without ``keep_parts``, for a call that has none).  ``bucket`` and ``table`` (buckets, 2h), both or neither: the
+    bias of attention_bucket_forward, a column per map, with the same rule for positions that take no part."""
+    graph, e = _rows_graph(row, indptr, indices)
+    return _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts)
+
+
+def attention_diff_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, q, k, v, lam, parts, lse, d_o, scale, bucket=None,
+                            table=None):
+    """[dq, dk, dv, d_lam] (and d_table with a bias) of attention_diff_forward; eid_t as in attention_bucket_backward."""
+    graph, e = _both_graphs(row, indptr, indices, col, indptr_t, eid_t, indices_t)
+    return _diff_backward(graph, e, q, k, v, lam, parts, lse, d_o, scale, bucket, table)
+
+
+def attention_diff_forward_planned(plan, q, k, v, lam, scale, bucket=None, table=None, keep_parts=True):
+    """attention_diff_forward on a plan of the row CSR."""
+    graph, e = _plan_rows(plan, q.size(0))
+    return _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts)
+
+
+def attention_diff_backward_planned(plan_r, plan_t, q, k, v, lam, parts, lse, d_o, scale, bucket=None, table=None):
+    """attention_diff_backward on plans of both orientations (plan_t with the transposed CSR's edge ids)."""
+    graph, e = _plan_both(plan_r, plan_t, q.size(0), k.size(0))
+    return _diff_backward(graph, e, q, k, v, lam, parts, lse, d_o, scale, bucket, table)

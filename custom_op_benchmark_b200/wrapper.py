@@ -16,6 +16,7 @@ from . import native_functions_if_built
 from .part_csr import partition_csr  # noqa: F401  (the reference wrapper re-exports it, wrapper.py:4)
 
 __all__ = ["SparseSoftmax", "MaskedMMCSR", "NodeMulEdge", "VectorSPMM", "GraphAttention", "GraphAttentionBias", "GraphAttentionPlanned",
+           "GraphAttentionBucket", "GraphAttentionBucketPlanned", "GraphAttentionDiff", "GraphAttentionDiffPlanned",
            "graph_attention", "partition_csr", "chunk_size"]
 
 chunk_size = 32  # wrapper.py:6
@@ -218,6 +219,107 @@ class GraphAttentionPlanned(Function):
         Q, K, V, o, lse = ctx.saved_tensors
         dq, dk, dv = _g.attention_backward_planned(ctx.plans[0], ctx.plans[1], Q, K, V, o, lse, d_o, ctx.scale)
         return None, None, dq, dk, dv, None
+
+
+class GraphAttentionBucket(Function):
+    """The attention layer with a learned bias by buckets in its scores (graphop.attention_bucket_forward):
+    ``apply(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, scale)``; ``bucket`` (e,) int32 by
+    row-CSR position, ``table`` (buckets, h).  Gradients for Q, K, V and table."""
+
+    @staticmethod
+    def apply(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, scale):
+        return _run(GraphAttentionBucket, "attention_bucket", row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket,
+                    table, scale)
+
+    @staticmethod
+    def forward(ctx, row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, scale):
+        o, lse = _g.attention_bucket_forward(row, indptr, indices, Q, K, V, bucket, table, scale)
+        ctx.save_for_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, o, lse)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        graph, (Q, K, V, bucket, table, o, lse) = ctx.saved_tensors[:7], ctx.saved_tensors[7:]
+        dq, dk, dv, dt = _g.attention_bucket_backward(*graph, Q, K, V, bucket, table, o, lse, d_o, ctx.scale)
+        return None, None, None, None, None, None, None, dq, dk, dv, None, dt, None
+
+
+class GraphAttentionBucketPlanned(Function):
+    """GraphAttentionBucket on graph plans: ``apply(plan_r, plan_t, Q, K, V, bucket, table, scale)``."""
+
+    @staticmethod
+    def apply(plan_r, plan_t, Q, K, V, bucket, table, scale):
+        native = _native()
+        if native is not None:
+            out = native.attention_bucket_planned(plan_r.native(), plan_t.native(), Q, K, V, bucket, table, scale)
+            if out is not None:
+                return out
+        return super(GraphAttentionBucketPlanned, GraphAttentionBucketPlanned).apply(plan_r, plan_t, Q, K, V, bucket, table, scale)
+
+    @staticmethod
+    def forward(ctx, plan_r, plan_t, Q, K, V, bucket, table, scale):
+        o, lse = _g.attention_bucket_forward_planned(plan_r, Q, K, V, bucket, table, scale)
+        ctx.save_for_backward(Q, K, V, bucket, table, o, lse)
+        ctx.plans, ctx.scale = (plan_r, plan_t), scale
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        dq, dk, dv, dt = _g.attention_bucket_backward_planned(*ctx.plans, *ctx.saved_tensors, d_o, ctx.scale)
+        return None, None, dq, dk, dv, None, dt, None
+
+
+class GraphAttentionDiff(Function):
+    """Differential attention (graphop.attention_diff_forward): ``apply(row, indptr, indices, col, indptr_t, eid_t, indices_t,
+    Q, K, V, lam, scale, bucket=None, table=None)``; Q (n, 2h, d), K (m, 2h, d), V (m, h, 2d), lam (h,), with ``bucket`` and
+    ``table`` (buckets, 2h) a bias for both maps.  Gradients for Q, K, V, lam and table."""
+
+    @staticmethod
+    def apply(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, lam, scale, bucket=None, table=None):
+        return _run(GraphAttentionDiff, "attention_diff", row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, lam, scale,
+                    bucket, table)
+
+    @staticmethod
+    def forward(ctx, row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, lam, scale, bucket=None, table=None):
+        o, lse, parts = _g.attention_diff_forward(row, indptr, indices, Q, K, V, lam, scale, bucket, table,
+                                                  keep_parts=any(ctx.needs_input_grad))
+        ctx.save_for_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, lam, parts, lse, bucket, table)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        graph, (Q, K, V, lam, parts, lse, bucket, table) = ctx.saved_tensors[:7], ctx.saved_tensors[7:]
+        dq, dk, dv, dl, *dt = _g.attention_diff_backward(*graph, Q, K, V, lam, parts, lse, d_o, ctx.scale, bucket, table)
+        return None, None, None, None, None, None, None, dq, dk, dv, dl, None, None, dt[0] if dt else None
+
+
+class GraphAttentionDiffPlanned(Function):
+    """GraphAttentionDiff on graph plans: ``apply(plan_r, plan_t, Q, K, V, lam, scale, bucket=None, table=None)``."""
+
+    @staticmethod
+    def apply(plan_r, plan_t, Q, K, V, lam, scale, bucket=None, table=None):
+        native = _native()
+        if native is not None:
+            out = native.attention_diff_planned(plan_r.native(), plan_t.native(), Q, K, V, lam, scale, bucket, table)
+            if out is not None:
+                return out
+        return super(GraphAttentionDiffPlanned, GraphAttentionDiffPlanned).apply(plan_r, plan_t, Q, K, V, lam, scale, bucket, table)
+
+    @staticmethod
+    def forward(ctx, plan_r, plan_t, Q, K, V, lam, scale, bucket=None, table=None):
+        o, lse, parts = _g.attention_diff_forward_planned(plan_r, Q, K, V, lam, scale, bucket, table,
+                                                          keep_parts=any(ctx.needs_input_grad))
+        ctx.save_for_backward(Q, K, V, lam, parts, lse, bucket, table)
+        ctx.plans, ctx.scale = (plan_r, plan_t), scale
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        Q, K, V, lam, parts, lse, bucket, table = ctx.saved_tensors
+        dq, dk, dv, dl, *dt = _g.attention_diff_backward_planned(*ctx.plans, Q, K, V, lam, parts, lse, d_o, ctx.scale, bucket, table)
+        return None, None, dq, dk, dv, dl, None, None, dt[0] if dt else None
 
 
 def graph_attention(row, indptr, eid, indices, col, indptr_t, eid_t, indices_t, Q, K, V, scale):
