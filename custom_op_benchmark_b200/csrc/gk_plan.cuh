@@ -186,6 +186,7 @@ inline int plan_build(const I* row, const I* indptr, const I* eid, const I* indi
   plan->eid = g.eid;
   plan->node_lo = node_lo;
   plan->node_deg = deg;
+  plan->node_first = first;
   {
     const unsigned aligning = (unsigned)((g.n_tiles + 256) / 256 < 4096 ? (g.n_tiles + 256) / 256 : 4096);
     const unsigned ranging = n_nodes > 0 && C > 0 ? (unsigned)((C + 255) / 256 < 8192 ? (C + 255) / 256 : 8192) : 0;

@@ -646,6 +646,18 @@ struct TermsCall {
   size_t node_bytes(long long n) const { return (size_t)n * H * row_d() * sizeof(T); }
 };
 
+// Defined in gk_terms_banded.cuh for bfloat16: the tensor-core kernels for dense-band graphs; GRAPHOP_ERR_UNSUPPORTED when the call is
+// not one they take.
+template <typename T>
+inline int banded_terms_forward(const graphop_plan_t*, const TermsCall<T>&, T*, T*, void*, void*, size_t, cudaStream_t) {
+  return GRAPHOP_ERR_UNSUPPORTED;
+}
+template <typename T>
+inline int banded_terms_backward(const graphop_plan_t*, const graphop_plan_t*, const TermsCall<T>&, const T*, const void*, const T*, T*,
+                                 T*, T*, T*, T*, void*, size_t, cudaStream_t) {
+  return GRAPHOP_ERR_UNSUPPORTED;
+}
+
 template <typename T>
 inline int terms_check(const TermsCall<T>& c, long long C, bool al, GeoPick* geo) {
   GK_TRY(check_sizes(C, c.E, c.n_dst, c.n_src, c.H, c.D));
@@ -690,6 +702,10 @@ inline int terms_forward(const GS& gs, long long C, const TermsCall<T>& c, T* o,
   if (!c.q || !c.k || !c.v || !gs.valid(true) || (c.diff && !c.lam) || (c.buckets && (!c.bucket || !c.table)))
     return GRAPHOP_ERR_INVALID_ARGUMENT;
   GK_TRY(check_ws(ws));
+  if constexpr (std::is_same_v<GS, FromPlan>) {
+    const int rc = banded_terms_forward<T>(gs.p, c, o, parts, lse, ws, wsb, st);
+    if (rc != GRAPHOP_ERR_UNSUPPORTED) return rc;
+  }
   Arena ar(ws, wsb);
   GraphView g;
   GK_TRY(gs(ar, c.n_dst, st, &g));
@@ -769,6 +785,10 @@ inline int terms_backward(const GS& gs_r, const GS& gs_c, bool has_eid_t, long l
       (c.diff && !c.lam) || (c.buckets && (!c.bucket || !c.table)) || !aligned_to(lse, c.maps() * sizeof(A)))
     return GRAPHOP_ERR_INVALID_ARGUMENT;
   GK_TRY(check_ws(ws));
+  if constexpr (std::is_same_v<GS, FromPlan>) {
+    const int rc = banded_terms_backward<T>(gs_r.p, gs_c.p, c, o, lse, dout, dq, dk, dv, d_table, d_lam, ws, wsb, st);
+    if (rc != GRAPHOP_ERR_UNSUPPORTED) return rc;
+  }
   Arena ar(ws, wsb);
   const int Hp = stat_heads(columns, (int)sizeof(A));
   auto* pd = (EdgePair<A>*)ar.take((size_t)c.E * Hp * sizeof(EdgePair<A>));   // survives both passes

@@ -184,6 +184,7 @@ typedef struct graphop_plan {
   const int32_t* tile_start; /* device, n_tiles + 1: first position of every work tile (GRAPHOP_PLAN_ROW_TILES) */
   int32_t tile;            /* cost per work tile the boundaries were made for */
   int32_t gather_repeats;  /* of up to 1024 evenly spaced positions, how many gather a row that another one gathers */
+  const int32_t* node_first; /* device, n_nodes: first position of every node that owns any */
 } graphop_plan_t;
 
 /* Bytes of device memory (256-byte aligned) a plan of these sizes needs. */

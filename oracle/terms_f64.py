@@ -145,7 +145,7 @@ def bounds(r, q, k, v, scale, dtype, bucket=None, table=None, staged=0.0):
         inside = (bucket >= 0) & (bucket < table.shape[0])
         b = bucket[inside].long()
         count = th.bincount(b, minlength=table.shape[0]).to(F64)[:, None]
-        out["d_table"] = add(table.shape, b, eg[inside]) + a * (count + 8) * add(table.shape, b, gs[inside]) + u * r["d_table"].abs()
+        out["d_table"] = add(table.shape, b, es_g[inside]) + a * (count + 8) * add(table.shape, b, gs[inside]) + u * r["d_table"].abs()
     return out
 
 

@@ -88,7 +88,10 @@ def test_training_step(name, g, diff, buckets, dt, idt, h, d):
         layer.table[2, 0] = -math.inf
         layer.table[4, -1] = th.finfo(dt).min
     layer.check(layer.step())
-    layer.check(layer.step(layer.plans()))
+    plans = layer.plans()
+    # a dense band in bfloat16 with 64 features per head of v: probabilities and score gradients enter the products as bfloat16
+    dense = dt == th.bfloat16 and layer.v.shape[2] == 64 and plans[0].dense_band
+    layer.check(layer.step(plans), th.finfo(dt).eps / 2 if dense else 0.0)
 
 
 @pytest.mark.parametrize("diff,buckets", KINDS, ids=KIND_IDS)
