@@ -91,7 +91,7 @@ UNTYPED = {
 
 
 # include/graphop_terms.h: the attention layers with learned score terms
-TERMS_BUCKET_FWD, TERMS_BUCKET_BWD, TERMS_DIFF_FWD, TERMS_DIFF_BWD, TERMS_RELATIVE = range(5)
+TERMS_BUCKET_FWD, TERMS_BUCKET_BWD, TERMS_DIFF_FWD, TERMS_DIFF_BWD = range(4)
 TERMS_SIGNATURES = {
     "attention_bucket_forward": [_P] * 3 + [_I64] + [_P] * 5 + [_INT, _DBL] + [_P] * 2 + [_I64] * 3 + [_INT] * 2 + _TAIL,
     "attention_bucket_backward": [_P] * 3 + [_I64] + [_P] * 4 + [_I64] + [_P] * 5 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 4
@@ -110,8 +110,8 @@ TERMS_PLANNED_SIGNATURES = {
 }
 TERMS_UNTYPED = {
     "graphop_terms_workspace_bytes": ([_INT, _I64, _I64] + [_INT] * 5, _SZ),
-    "graphop_relative_buckets_i32": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64] + _TAIL, _INT),
-    "graphop_relative_buckets_i64": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64] + _TAIL, _INT),
+    "graphop_relative_buckets_i32": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64, _P], _INT),
+    "graphop_relative_buckets_i64": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64, _P], _INT),
     "graphop_relative_buckets_planned_i32": ([_PP] + [_P] * 3 + [_INT] * 2 + [_P] * 2, _INT),
     "graphop_relative_buckets_planned_i64": ([_PP] + [_P] * 3 + [_INT] * 2 + [_P] * 2, _INT),
 }

@@ -742,7 +742,9 @@ struct TermsBackward : GraphNode {
   }
 };
 
-Tensor terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, double scale) {
+// o; lse and parts as the entry point leaves them.  `keep`: parts whether or not a gradient will be asked for.
+struct TermsOutputs { Tensor o, lse, parts; };
+TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, double scale, bool track, bool keep) {
   const int64_t e = graph.edges();
   int ib = 4;
   if (!graph.planned()) {
@@ -753,13 +755,13 @@ Tensor terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, d
   const TermsShape s = check_terms(x, diff, e);
   Call c(x.q);
   bool grads = false;
-  if (c10::GradMode::is_enabled())
+  if (track && c10::GradMode::is_enabled())
     for (const Tensor* t : {&x.q, &x.k, &x.v, &x.lam, &x.table}) grads = grads || (t->defined() && t->requires_grad());
   Tensor o = at::empty(x.v.dim() == 3 ? std::vector<int64_t>{s.n, x.v.size(1), x.v.size(2)} : std::vector<int64_t>{s.n, x.v.size(1)},
                        x.q.options());
   const int64_t maps = diff ? 2 * s.H : s.H;
   Tensor lse = at::empty({s.n, maps}, x.q.options().dtype(s.elem == 1 ? at::kDouble : at::kFloat)), parts;
-  if (diff && grads) parts = at::empty({s.n, s.H, 2, 2 * s.D}, x.q.options());
+  if (diff && (grads || keep)) parts = at::empty({s.n, s.H, 2, 2 * s.D}, x.q.options());
   terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_FWD : GRAPHOP_TERMS_BUCKET_FWD, e, s, x.q, ib);
   const auto typed = [&](auto* y, auto&& call) {
     using E = std::remove_pointer_t<decltype(y)>;
@@ -792,7 +794,7 @@ Tensor terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, d
   }
   check_status(rc, diff ? (graph.planned() ? "attention_diff_forward_planned" : "attention_diff_forward")
                         : (graph.planned() ? "attention_bucket_forward_planned" : "attention_bucket_forward"));
-  const auto keep = [&](TermsBackward& n) {
+  const auto save = [&](TermsBackward& n) {
     n.diff = diff;
     n.rows = graph.rows;
     n.cols = graph.cols;
@@ -804,10 +806,10 @@ Tensor terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, d
       for (const Tensor& t : graph.t) n.save(t);
   };
   if (grads) {
-    if (diff) record<TermsBackward>({x.q, x.k, x.v, x.lam, x.table}, o, keep);
-    else record<TermsBackward>({x.q, x.k, x.v, x.table}, o, keep);
+    if (diff) record<TermsBackward>({x.q, x.k, x.v, x.lam, x.table}, o, save);
+    else record<TermsBackward>({x.q, x.k, x.v, x.table}, o, save);
   }
-  return o;
+  return {o, lse, parts};
 }
 
 Result terms_on_tables(std::initializer_list<Tensor> index, const TermsInputs& x, bool diff, double scale) {
@@ -816,7 +818,7 @@ Result terms_on_tables(std::initializer_list<Tensor> index, const TermsInputs& x
   for (const Tensor& t : graph.t)
     if (left_to_python({&t})) return c10::nullopt;
   if (left_to_python({&x.q, &x.k, &x.v, &x.lam, &x.bucket, &x.table})) return c10::nullopt;
-  return terms_forward(graph, x, diff, scale);
+  return terms_forward(graph, x, diff, scale, true, false).o;
 }
 Result terms_on_plans(const PlanHandle& plan_r, const PlanHandle& plan_t, const TermsInputs& x, bool diff, double scale) {
   if (left_to_python({&x.q, &x.k, &x.v, &x.lam, &x.bucket, &x.table})) return c10::nullopt;
@@ -824,7 +826,7 @@ Result terms_on_plans(const PlanHandle& plan_r, const PlanHandle& plan_t, const 
   TermsGraph graph;
   graph.rows = plan_r.graph;
   graph.cols = plan_t.graph;
-  return terms_forward(graph, x, diff, scale);
+  return terms_forward(graph, x, diff, scale, true, false).o;
 }
 Result attention_bucket(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Later& col, const Later& indptr_t,
                         const Later& eid_t, const Later& indices_t, const Tensor& q, const Tensor& k, const Tensor& v, const Later& bucket,
@@ -845,6 +847,91 @@ Result attention_bucket_planned_(const PlanHandle& plan_r, const PlanHandle& pla
 Result attention_diff_planned_(const PlanHandle& plan_r, const PlanHandle& plan_t, const Tensor& q, const Tensor& k, const Tensor& v,
                                const Tensor& lam, double scale, const Later& bucket, const Later& table) {
   return terms_on_plans(plan_r, plan_t, {q, k, v, lam, given(bucket), given(table)}, true, scale);
+}
+
+// graphop.py's functions of the same names: no autograd
+using Values = std::tuple<Tensor, Tensor, c10::optional<Tensor>>;
+TermsGraph rows_only(const Tensor& row, const Tensor& indptr, const Tensor& indices) {
+  TermsGraph graph;
+  graph.t[0] = row; graph.t[1] = indptr; graph.t[2] = indices;
+  return graph;
+}
+TermsGraph rows_only(const PlanHandle& plan, const Tensor& q) {
+  check_terms_plan(plan, q.defined() && q.dim() ? q.size(0) : 0);
+  TermsGraph graph;
+  graph.rows = plan.graph;
+  return graph;
+}
+std::tuple<Tensor, Tensor> attention_bucket_forward_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Tensor& q,
+                                                     const Tensor& k, const Tensor& v, const Later& bucket, const Later& table, double scale) {
+  const TermsOutputs r = terms_forward(rows_only(row, indptr, indices), {q, k, v, Tensor(), given(bucket), given(table)}, false, scale, false, false);
+  return {r.o, r.lse};
+}
+std::tuple<Tensor, Tensor> attention_bucket_forward_plan(const PlanHandle& plan, const Tensor& q, const Tensor& k, const Tensor& v,
+                                                         const Later& bucket, const Later& table, double scale) {
+  const TermsOutputs r = terms_forward(rows_only(plan, q), {q, k, v, Tensor(), given(bucket), given(table)}, false, scale, false, false);
+  return {r.o, r.lse};
+}
+Values diff_values(const TermsOutputs& r) {
+  return {r.o, r.lse, r.parts.defined() ? c10::optional<Tensor>(r.parts) : c10::nullopt};
+}
+Values attention_diff_forward_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Tensor& q, const Tensor& k,
+                               const Tensor& v, const Tensor& lam, double scale, const Later& bucket, const Later& table, bool keep_parts) {
+  return diff_values(terms_forward(rows_only(row, indptr, indices), {q, k, v, lam, given(bucket), given(table)}, true, scale, false, keep_parts));
+}
+Values attention_diff_forward_plan(const PlanHandle& plan, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam,
+                                   double scale, const Later& bucket, const Later& table, bool keep_parts) {
+  return diff_values(terms_forward(rows_only(plan, q), {q, k, v, lam, given(bucket), given(table)}, true, scale, false, keep_parts));
+}
+
+// both ends' positions, checked as graphop._positions does; `type`: the index type, if the call has one
+c10::optional<at::ScalarType> check_positions(const Tensor& dst, const Tensor& src, int64_t n_dst, c10::optional<at::ScalarType> type,
+                                              const at::Device& device) {
+  const std::pair<const Tensor*, const char*> both[2] = {{&dst, "dst_pos"}, {&src, "src_pos"}};
+  for (const auto& [t, name] : both) {
+    if (!t->defined()) continue;
+    check_input(*t, name);
+    const bool index = t->scalar_type() == at::kInt || t->scalar_type() == at::kLong;
+    if (t->dim() != 1 || !index || (type && t->scalar_type() != *type))
+      fail(std::string(name) + " must be a one-dimensional tensor of the call's index type");
+    if (t->device() != device) fail(std::string(name) + " must be on the graph's device");
+    if (t == &dst && n_dst >= 0 && t->numel() < n_dst) fail(std::string(name) + " must hold a position for every node");
+    type = t->scalar_type();
+  }
+  return type;
+}
+Tensor relative_buckets_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const std::vector<int64_t>& limits, bool both,
+                         const Later& dst_in, const Later& src_in) {
+  const Tensor dst = given(dst_in), src = given(src_in);
+  check_input(row, "row"); check_input(indptr, "indptr"); check_input(indices, "indices");
+  const int ib = index_bytes_of({&row, &indptr, &indices});
+  check_chunks(row, indptr);
+  check_positions(dst, src, -1, indices.scalar_type(), indices.device());
+  Call c(indices);
+  Tensor out = at::empty({indices.size(0)}, indices.options().dtype(at::kInt));
+  const auto call = [&](auto* i, auto&& f) {
+    using I = std::remove_pointer_t<decltype(i)>;
+    return f(owners<I>(row, indptr), (const I*)ptr<I>(indptr), (const I*)ptr<I>(indices), row.size(0), (const I*)ptr<I>(dst),
+             (const I*)ptr<I>(src), limits.data(), (int)limits.size(), (int)both, out.data_ptr<int32_t>(), indices.size(0), raw(c.stream));
+  };
+  check_status(ib == 8 ? call((int64_t*)nullptr, graphop_relative_buckets_i64) : call((int32_t*)nullptr, graphop_relative_buckets_i32),
+               "relative_buckets");
+  return out;
+}
+Tensor relative_buckets_plan(const PlanHandle& plan, const std::vector<int64_t>& limits, bool both, const Later& dst_in, const Later& src_in,
+                             const Tensor& like) {
+  const Tensor dst = given(dst_in), src = given(src_in);
+  const graphop_plan_t* p = &plan.graph->plan;
+  const auto type = check_positions(dst, src, p->n_nodes, c10::nullopt, like.device());
+  Call c(like);
+  Tensor out = at::empty({p->n_edges}, like.options().dtype(at::kInt));
+  int32_t* to = out.data_ptr<int32_t>();
+  check_status(type == at::kLong ? graphop_relative_buckets_planned_i64(p, ptr<int64_t>(dst), ptr<int64_t>(src), limits.data(), (int)limits.size(),
+                                                                        (int)both, to, raw(c.stream))
+                                 : graphop_relative_buckets_planned_i32(p, ptr<int32_t>(dst), ptr<int32_t>(src), limits.data(), (int)limits.size(),
+                                                                        (int)both, to, raw(c.stream)),
+               "relative_buckets_planned");
+  return out;
 }
 
 // ---- graph preparation: graphop.py's functions of the same names ---------------------------
@@ -929,6 +1016,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_bucket_planned", &attention_bucket_planned_, free_gil());
   m.def("attention_diff", &attention_diff, free_gil());
   m.def("attention_diff_planned", &attention_diff_planned_, free_gil());
+  m.def("attention_bucket_forward", &attention_bucket_forward_, free_gil());
+  m.def("attention_bucket_forward_planned", &attention_bucket_forward_plan, free_gil());
+  m.def("attention_diff_forward", &attention_diff_forward_, free_gil());
+  m.def("attention_diff_forward_planned", &attention_diff_forward_plan, free_gil());
+  m.def("relative_buckets", &relative_buckets_, free_gil());
+  m.def("relative_buckets_planned", &relative_buckets_plan, free_gil());
   m.def("partition_csr", &partition_csr, free_gil());
   m.def("transpose_csr", &transpose_csr, free_gil());
   m.def("plan_build", &plan_build, free_gil());

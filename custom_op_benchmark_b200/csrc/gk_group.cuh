@@ -425,7 +425,10 @@ group_walk_kernel(const __grid_constant__ Op op, const __grid_constant__ WalkArg
       for (int k = 0; k < Op::kHeads; ++k) {
         const bool live = o >= 0 && k < per && k < pieces;
         const int ph = live ? hb * per + k : 0;
-        if constexpr (Op::kComputed) { raw[k] = op.raw_scalar(ph, e, live); continue; }
+        if constexpr (Op::kComputed) {
+          if (k < per) raw[k] = op.raw_scalar(ph, e, live);
+          continue;
+        }
         const void* src = op.scalar_of(op.parts == 1 ? ph : ph / op.parts, live ? o : 0, live ? e : 0);
         if constexpr (SC == 2) held[k] = live ? __ldg(reinterpret_cast<const uint16_t*>(src)) : (uint16_t)0;
         else cp_async_slot<SC>(tab + lane * ENTRY + k * SC, src, live);
@@ -434,8 +437,10 @@ group_walk_kernel(const __grid_constant__ Op op, const __grid_constant__ WalkArg
   };
   auto publish_scalars = [&](unsigned tab) {
     if constexpr (Op::kComputed) {
+      const int per = op.block_heads();
 #pragma unroll
-      for (int k = 0; k < Op::kHeads; ++k) op.put_scalar(tab + lane * ENTRY + k * SC, raw[k]);
+      for (int k = 0; k < Op::kHeads; ++k)
+        if (k < per) op.put_scalar(tab + lane * ENTRY + k * SC, raw[k]);
     } else if constexpr (SC == 2) {
 #pragma unroll
       for (int k = 0; k < Op::kHeads; ++k)

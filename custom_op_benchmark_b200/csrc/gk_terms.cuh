@@ -519,7 +519,9 @@ struct TermsSumPairs : SumAttnPairs<GEO> {
 // sums by bucket: out[b, h] = sign * sum of x[j, h] over the rows j of bucket b (bucket null: all rows are bucket 0)
 // ---------------------------------------------------------------------------------------
 // A stream of `lanes` threads, one head each, adds a contiguous range of rows into a table of its own in shared memory, one row
-// after the other; the streams' tables, and then the blocks', are added up in order.  No atomics: the same bits every time.
+// after the other; the streams' tables, and then the blocks', are added up in order.  No atomics: the same bits every time.  What takes
+// the time is waiting for rows, as the private tables leave a few hundred threads per SM: kBatch rows are asked for at once, and the
+// next ones before the last are added (4.5M edges, 4 heads, 128 buckets: 84 us with batches of four, none ahead).
 struct BucketSum {
   const int32_t* bucket;
   const PlanHeader* hdr;      // the rows are positions: only those that a chunk covers count; null: all of them
@@ -527,6 +529,7 @@ struct BucketSum {
   int col_stride, columns;    // columns (heads) of x
   int buckets, per, streams, lanes;   // per: columns of a block (blockIdx.y counts such blocks)
 };
+constexpr int kBatch = 8;
 template <typename A>
 __global__ void __launch_bounds__(256)
 bucket_sum_kernel(const A* __restrict__ x, const BucketSum a, double* __restrict__ partial) {
@@ -534,32 +537,39 @@ bucket_sum_kernel(const A* __restrict__ x, const BucketSum a, double* __restrict
   A* cells = reinterpret_cast<A*>(gk_ring);
   const int tid = threadIdx.x, stream = tid / a.lanes, col = tid - stream * a.lanes, c0 = blockIdx.y * a.per;
   const int cols = a.columns - c0 < a.per ? a.columns - c0 : a.per, size = a.buckets * a.per;
-  for (int i = tid; i < a.streams * size; i += blockDim.x) cells[i] = A(0);
-  __syncthreads();
   long long lo = 0, hi = a.rows;
   if (a.hdr) {
     lo = a.hdr->cover_lo > 0 ? a.hdr->cover_lo : 0;
     hi = a.hdr->cover_hi < a.rows ? a.hdr->cover_hi : a.rows;
   }
   const long long all = (long long)gridDim.x * a.streams, each = hi > lo ? (hi - lo + all - 1) / all : 0;
-  const long long j0 = lo + ((long long)blockIdx.x * a.streams + stream) * each, j1 = j0 + each < hi ? j0 + each : hi;
-  if (stream < a.streams && col < cols) {
-    A* mine = cells + (size_t)stream * size + col;
-    const A* src = x + (long long)(c0 + col) * a.col_stride;
-    constexpr int U = 4;
-    for (long long j = j0; j < j1; j += U) {
-      int b[U];
-      A g[U];
+  const bool works = stream < a.streams && col < cols;
+  const long long j0 = lo + ((long long)blockIdx.x * a.streams + stream) * each, j1 = !works ? j0 : j0 + each < hi ? j0 + each : hi;
+  const A* src = x + (long long)(c0 + (works ? col : 0)) * a.col_stride;
+  int b0[kBatch], b1[kBatch];
+  A g0[kBatch], g1[kBatch];
+  const auto ask = [&](int (&b)[kBatch], A (&g)[kBatch], long long j) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool in = j + u < j1;
-        b[u] = !in ? -1 : a.bucket ? __ldg(a.bucket + j + u) : 0;
-        g[u] = in ? __ldg(src + (j + u) * a.row_stride) : A(0);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if ((unsigned)b[u] < (unsigned)a.buckets) mine[(size_t)b[u] * a.per] += g[u];
+    for (int u = 0; u < kBatch; ++u) {
+      const bool in = j + u < j1;
+      b[u] = !in ? -1 : a.bucket ? __ldg(a.bucket + j + u) : 0;
+      g[u] = in ? __ldg(src + (j + u) * a.row_stride) : A(0);
     }
+  };
+  ask(b0, g0, j0);
+  for (int i = tid; i < a.streams * size; i += blockDim.x) cells[i] = A(0);
+  __syncthreads();
+  A* mine = cells + (size_t)stream * size + col;
+  const auto add = [&](const int (&b)[kBatch], const A (&g)[kBatch]) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if ((unsigned)b[u] < (unsigned)a.buckets) mine[(size_t)b[u] * a.per] += g[u];
+  };
+  for (long long j = j0; j < j1; j += 2 * kBatch) {
+    ask(b1, g1, j + kBatch);
+    add(b0, g0);
+    ask(b0, g0, j + 2 * kBatch);
+    add(b1, g1);
   }
   __syncthreads();
   double* out = partial + (size_t)blockIdx.x * a.buckets * a.columns;
@@ -571,23 +581,28 @@ bucket_sum_kernel(const A* __restrict__ x, const BucketSum a, double* __restrict
     out[(size_t)b * a.columns + c0 + c] = s;
   }
 }
+// The blocks' partials of 8 cells per block of this kernel: 32 threads per cell take every 32nd block, then add up by halves.
 template <typename T>
 __global__ void __launch_bounds__(256)
 bucket_total_kernel(const double* __restrict__ partial, int blocks, int cells, double sign, T* __restrict__ out) {
-  __shared__ double s_part[8][32];
-  const int c = threadIdx.x & 31, slice = threadIdx.x >> 5, i = blockIdx.x * 32 + c;
+  __shared__ double s_part[32][9];
+  const int c = threadIdx.x & 7, slice = threadIdx.x >> 3, i = blockIdx.x * 8 + c;
   double s = 0;
-  if (i < cells)
-    for (int b = slice; b < blocks; b += 8) s += partial[(size_t)b * cells + i];
+  if (i < cells) {
+#pragma unroll 8
+    for (int b = slice; b < blocks; b += 32) s += partial[(size_t)b * cells + i];
+  }
   s_part[slice][c] = s;
   __syncthreads();
-  if (slice == 0 && i < cells) {
-    for (int k = 1; k < 8; ++k) s += s_part[k][c];
-    out[i] = from_acc<T>((typename AccOf<T>::type)(sign * s));
-  }
+  const int lane = threadIdx.x & 31, cell = threadIdx.x >> 5;   // a warp per cell
+  s = s_part[lane][cell];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+  const int at = blockIdx.x * 8 + cell;
+  if (lane == 0 && at < cells) out[at] = from_acc<T>((typename AccOf<T>::type)(sign * s));
 }
 
-constexpr int kSumSmem = 64 * 1024;             // of a block: three of them per SM
+constexpr int kSumSmem = 32 * 1024;             // of a block
 constexpr int kMostBuckets = 16384;
 // How a sum by bucket is launched.
 struct BucketShape { int lanes, per, streams, blocks, col_blocks; };
@@ -602,9 +617,9 @@ inline BucketShape bucket_shape(long long rows, int columns, int buckets, int ac
   s.streams = 256 / s.lanes;
   if (s.streams > fit) s.streams = fit < 1 ? 1 : (int)fit;
   s.col_blocks = (columns + s.per - 1) / s.per;
-  // a stream has 32 rows at least, and the chip three blocks per SM at most
-  const long long want = rows / (32ll * s.streams) + 1;
-  s.blocks = want < 3 * 148 ? (int)want : 3 * 148;
+  // a stream has two batches at least, and the chip four blocks per SM at most, over all blocks of columns: their tables are added up
+  const long long want = rows / (2ll * kBatch * s.streams) + 1, most = 4 * 148 / s.col_blocks + 1;
+  s.blocks = (int)(want < most ? want : most);
   return s;
 }
 inline size_t bucket_sum_bytes(long long rows, int columns, int buckets, int acc) {
@@ -623,7 +638,7 @@ inline int run_bucket_sum(Arena& ar, const A* x, long long rows, long long row_s
   bucket_sum_kernel<A><<<dim3(s.blocks, s.col_blocks), threads, smem, st>>>(x, a, partial);
   GK_LAUNCHED("bucket_sum");
   const int cells = buckets * columns;
-  bucket_total_kernel<T><<<(cells + 31) / 32, 256, 0, st>>>(partial, s.blocks, cells, sign, out);
+  bucket_total_kernel<T><<<(cells + 7) / 8, 256, 0, st>>>(partial, s.blocks, cells, sign, out);
   GK_LAUNCHED("bucket_total");
   return GRAPHOP_OK;
 }
@@ -658,6 +673,18 @@ inline int banded_terms_backward(const graphop_plan_t*, const graphop_plan_t*, c
   return GRAPHOP_ERR_UNSUPPORTED;
 }
 
+// The geometry of a row: the plain layer's, but blocks of as many heads as divide their number, where that makes every lane own whole
+// slots known at compile time.
+template <typename T>
+inline GeoPick terms_geo(int H, int D) {
+  const GeoPick p = pick_geo(H, D, sizeof(T), 16, false);
+  if (p.LT || (H & (H - 1)) == 0) return p;
+  GeoPick q = pick_geo(H & -H, D, sizeof(T), 16, false);   // the largest power of two in H
+  if (!q.LT) return p;
+  q.nhb = H / (q.G / q.L);
+  return q;
+}
+
 template <typename T>
 inline int terms_check(const TermsCall<T>& c, long long C, bool al, GeoPick* geo) {
   GK_TRY(check_sizes(C, c.E, c.n_dst, c.n_src, c.H, c.D));
@@ -665,7 +692,9 @@ inline int terms_check(const TermsCall<T>& c, long long C, bool al, GeoPick* geo
   if (c.buckets < (c.diff ? 0 : 1)) return GRAPHOP_ERR_INVALID_ARGUMENT;
   if (c.buckets > kMostBuckets) return GRAPHOP_ERR_UNSUPPORTED;
   if (!is_pow2(c.D * (int)sizeof(T) / 16) || c.D * (int)sizeof(T) % 16) return GRAPHOP_ERR_UNSUPPORTED;
-  return attention_shape_ok<T>(c.H, c.row_d(), al, geo) ? GRAPHOP_OK : GRAPHOP_ERR_UNSUPPORTED;
+  if (!attention_shape_ok<T>(c.H, c.row_d(), al, geo)) return GRAPHOP_ERR_UNSUPPORTED;
+  *geo = terms_geo<T>(c.H, c.row_d());
+  return GRAPHOP_OK;
 }
 inline bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -732,7 +761,7 @@ inline int run_terms_src(Arena& ar, const GraphView& g, const TermsCall<T>& c, c
                          T* dv, cudaStream_t st) {
   const int H = c.H * c.maps(), D = c.D;
   const long long table = (long long)c.node_bytes(c.n_dst);
-  const GeoPick s = pick_geo(H, D, sizeof(T), 16, false);
+  const GeoPick s = terms_geo<T>(H, D);
   const auto ring = [&](int only, int most) -> int {
     return dispatch_geo<T, false, true>(s, [&](auto tag) -> int {
       TermsBwdSrc<typename decltype(tag)::type> op;

@@ -61,45 +61,62 @@ __device__ __forceinline__ void band_reduce(int lo, int deg, int part, bool writ
 }
 
 // ids[tile][column / kC][row][column % kC], kC columns per thread of the tile's kernel.  eid: the transposed CSR's edge ids, or null.
-constexpr int kIdRows = 16;   // rows of a tile per block: 128 tiles of a short sequence alone would leave most of the chip idle
-template <int kC>
-__global__ void __launch_bounds__(256)
-band_ids_kernel(const int32_t* __restrict__ node_lo, const int32_t* __restrict__ node_deg, const int32_t* __restrict__ node_first,
-                const int32_t* __restrict__ eid, const int32_t* __restrict__ bucket, int buckets, long long n, int pitch,
-                unsigned char* __restrict__ ids) {
+// One orientation; a launch takes both where the backward needs both (blockIdx.z).
+struct BandIds {
+  const int32_t *node_lo, *node_deg, *node_first, *eid;
+  long long n;
+  int pitch, per;        // per: kC
+  unsigned char* ids;
+};
+// A warp per row, 32 columns at a time, one per lane: neighbouring positions in one load, and the loads of all of them at once.
+// Bound by the chain node - position - (edge id -) bucket, which every warp goes through once.
+static __global__ void __launch_bounds__(256)
+band_ids_kernel(const __grid_constant__ BandIds a0, const __grid_constant__ BandIds a1, const int32_t* __restrict__ bucket, int buckets) {
+  const BandIds& a = blockIdx.z ? a1 : a0;
   __shared__ int s_min[4], s_top[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long r0 = (long long)blockIdx.x * kTileM;
+  if (r0 >= a.n) return;
+  const int row = blockIdx.y * 8 + warp;
+  const long long r = r0 + row;
+  int deg = 0, lo = 0, first = 0;
+  if (r < a.n) {
+    deg = a.node_deg[r];
+    lo = a.node_lo[r];
+    first = a.node_first[r];
+  }
   if (warp < 4) {
-    int lo = INT_MAX, deg = 0;
-    if (r0 + tid < n) {
-      deg = node_deg[r0 + tid];
-      if (deg > 0) lo = node_lo[r0 + tid];
+    int l = INT_MAX, d = 0;
+    if (r0 + tid < a.n) {
+      d = a.node_deg[r0 + tid];
+      l = d > 0 ? a.node_lo[r0 + tid] : INT_MAX;
     }
-    band_reduce<4>(lo, deg, warp, lane == 0, s_min, s_top);
+    band_reduce<4>(l, d, warp, lane == 0, s_min, s_top);
   }
   __syncthreads();
   const int kmin = min(min(s_min[0], s_min[1]), min(s_min[2], s_min[3]));
-  unsigned char* out = ids + (size_t)blockIdx.x * pitch * kTileM;
-  for (int row = blockIdx.y * kIdRows + warp; row < (blockIdx.y + 1) * kIdRows; row += 8) {
-    const long long r = r0 + row;
-    const int deg = r < n ? node_deg[r] : 0;
-    const int jlo = deg > 0 ? node_lo[r] - kmin : 0;
-    const int first = deg > 0 ? node_first[r] : 0;
-    for (int c = lane * 4; c < pitch; c += 128) {
-      unsigned w = 0;
+  unsigned char* out = a.ids + (size_t)blockIdx.x * a.pitch * kTileM;
+  const int jlo = deg > 0 ? lo - kmin : 0;
+  constexpr int kSteps = kSpan / 32;
+  int at[kSteps], b[kSteps];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = c + i - jlo;
-        unsigned id = kNoPart;
-        if (k >= 0 && k < deg) {
-          const unsigned b = (unsigned)__ldg(bucket + (eid ? __ldg(eid + first + k) : first + k));
-          if (b < (unsigned)buckets) id = b;
-        }
-        w |= id << (8 * i);
-      }
-      *reinterpret_cast<unsigned*>(out + (size_t)(c / kC) * kC * kTileM + row * kC + c % kC) = w;
-    }
+  for (int i = 0; i < kSteps; ++i) {
+    const int k = i * 32 + lane - jlo;
+    at[i] = k >= 0 && k < deg ? first + k : -1;
+  }
+  if (a.eid) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      if (at[i] >= 0) at[i] = __ldg(a.eid + at[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) b[i] = at[i] >= 0 ? __ldg(bucket + at[i]) : -1;
+  const int shift = a.per == 32 ? 5 : 4;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int c = i * 32 + lane;
+    if (c < a.pitch)
+      out[(((size_t)(c >> shift) * kTileM + row) << shift) + (c & (a.per - 1))] = (unsigned)b[i] < (unsigned)buckets ? b[i] : kNoPart;
   }
 }
 
@@ -845,26 +862,34 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------------------------------------
 // dT: sums of g by bucket, over the tiles' elements in the threads' order
 // ---------------------------------------------------------------------------------------------------------
-// grid: (blocks, H * maps).  A thread takes pieces of 32 elements (a row's of one column group), every gridDim.x * blockDim.x'th,
-// into a table of its own: cell b of thread t at b * blockDim.x + t, so that a warp's 32 cells lie in 32 banks.
+// grid: (blocks, H * maps).  A thread takes 8 elements at a time, so that a warp's loads are whole lines, and asks for kAhead such
+// pieces at once; they go into a table of its own, cell b of thread t at b * blockDim.x + t: a warp's 32 cells lie in 32 banks.
+// Bound by reading the gradients and, once per head, the ids.
 static __global__ void __launch_bounds__(128)
-band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const __nv_bfloat16* __restrict__ g, long long pieces, int buckets,
+band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const __nv_bfloat16* __restrict__ g, long long elements, int buckets,
                        int columns, double* __restrict__ partial) {
   extern __shared__ float cells[];
+  constexpr int kAhead = 4;
   const int tid = threadIdx.x, nt = blockDim.x, column = blockIdx.y;
+  const long long pieces = elements / 8, stride = (long long)gridDim.x * nt;
+  const uint2* idp = reinterpret_cast<const uint2*>(ids);
+  const uint4* src = reinterpret_cast<const uint4*>(g + (size_t)column * elements);
   for (int b = 0; b < buckets; ++b) cells[b * nt + tid] = 0.f;
-  const uint4* src = reinterpret_cast<const uint4*>(g + (size_t)column * pieces * 32);
-  for (long long i = (long long)blockIdx.x * nt + tid; i < pieces; i += (long long)gridDim.x * nt) {
-    const uint4* idp = reinterpret_cast<const uint4*>(ids) + i * 2;
-    const uint4 id[2] = {__ldg(idp), __ldg(idp + 1)};
-    if ((id[0].x & id[0].y & id[0].z & id[0].w & id[1].x & id[1].y & id[1].z & id[1].w) == 0xffffffffu) continue;   // nothing takes part
+  for (long long i = (long long)blockIdx.x * nt + tid; i < pieces; i += kAhead * stride) {
+    uint2 id[kAhead];
+    uint4 w[kAhead];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 w = __ldg(src + i * 4 + q);
-      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+    for (int k = 0; k < kAhead; ++k) id[k] = i + k * stride < pieces ? __ldg(idp + i + k * stride) : make_uint2(0xffffffffu, 0xffffffffu);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if ((id[k].x & id[k].y) != 0xffffffffu) w[k] = __ldg(src + i + k * stride);   // else nothing takes part
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if ((id[k].x & id[k].y) == 0xffffffffu) continue;
+      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w[k]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const unsigned b = id_at(id[q >> 1], (q & 1) * 8 + j);
+        const unsigned b = ((j < 4 ? id[k].x : id[k].y) >> (8 * (j & 3))) & 255u;
         const float v = (j & 1) ? __high2float(x[j >> 1]) : __low2float(x[j >> 1]);
         if (b < (unsigned)buckets) cells[b * nt + tid] += v;
       }
@@ -900,11 +925,13 @@ inline bool band_plan_ok(const graphop_plan_t* plan, long long n, int H) {
   return (plan->flags & GRAPHOP_PLAN_DENSE_BAND) && plan->band_span > 0 && plan->band_span <= kSpan && plan->node_lo && plan->node_deg &&
          plan->node_first && n >= 1 && n <= plan->n_nodes && H <= 65535;
 }
-template <int kC>
-inline int run_band_ids(const graphop_plan_t* plan, const int32_t* eid, const int32_t* bucket, int buckets, long long n, int pitch,
-                        unsigned char* ids, cudaStream_t st) {
-  band_ids_kernel<kC><<<dim3((unsigned)band_tiles_of(n), kTileM / kIdRows), 256, 0, st>>>(plan->node_lo, plan->node_deg, plan->node_first,
-                                                                                         eid, bucket, buckets, n, pitch, ids);
+inline BandIds band_ids_of(const graphop_plan_t* plan, const int32_t* eid, long long n, int per, unsigned char* ids) {
+  return BandIds{plan->node_lo, plan->node_deg, plan->node_first, eid, n, band_pitch(plan), per, ids};
+}
+// a1: null, or the other orientation
+inline int run_band_ids(const BandIds& a0, const BandIds* a1, const int32_t* bucket, int buckets, cudaStream_t st) {
+  const long long tiles = band_tiles_of(a1 && a1->n > a0.n ? a1->n : a0.n);
+  band_ids_kernel<<<dim3((unsigned)tiles, kTileM / 8, a1 ? 2 : 1), 256, 0, st>>>(a0, a1 ? *a1 : a0, bucket, buckets);
   GK_LAUNCHED("band_ids");
   return GRAPHOP_OK;
 }
@@ -931,7 +958,7 @@ inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat
     return GRAPHOP_ERR_UNSUPPORTED;
   static std::atomic<bool> configured[64];
   GK_TRY(allow_smem(terms_forward_kernel<kMaps, kBucket>, L::kBytes, configured));
-  if (kBucket) GK_TRY(run_band_ids<32>(plan, nullptr, c.bucket, c.buckets, c.n_dst, pitch, const_cast<unsigned char*>(t.ids), st));
+  if (kBucket) GK_TRY(run_band_ids(band_ids_of(plan, nullptr, c.n_dst, 32, const_cast<unsigned char*>(t.ids)), nullptr, c.bucket, c.buckets, st));
   t.table = c.table; t.lam = c.lam; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan->node_lo; t.node_deg = plan->node_deg;
   t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.o = o; t.parts = parts; t.lse = (float*)lse;
   terms_forward_kernel<kMaps, kBucket><<<dim3((unsigned)tiles, (unsigned)c.H), kThreads, L::kBytes, st>>>(mq, mk, mv, t);
@@ -948,10 +975,12 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   using LS = BwdLayout<true, kMaps>;
   const int pitch = band_pitch(plan_r), pitch_t = band_pitch(plan_t), columns = c.H * kMaps;
   const long long tiles = band_tiles_of(c.n_dst), tiles_t = band_tiles_of(c.n_src), pieces = tiles * pitch / 32 * kTileM;
-  // dT's sums: a block has a table per thread, so many threads that four blocks share an SM, or one has it
+  // dT's sums: a block has a table per thread; as many blocks as share the SMs' memory, a piece or more for every thread
   int threads = 128;
   while (threads > 32 && (size_t)c.buckets * threads * sizeof(float) > 56 * 1024) threads >>= 1;
-  long long blocks = (4 * 148 + columns - 1) / columns;
+  long long per_sm = kBucket ? 200 * 1024 / ((long long)c.buckets * threads * (long long)sizeof(float) + 1024) : 1;
+  if (per_sm > 8) per_sm = 8;
+  long long blocks = (per_sm * 148 + columns - 1) / columns;
   if (blocks > pieces / threads + 1) blocks = pieces / threads + 1;
 
   TermsTile t{};
@@ -980,8 +1009,8 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   GK_TRY(allow_smem(terms_backward_kernel<false, kMaps, kBucket>, LD::kBytes, configured));
   GK_TRY(allow_smem(terms_backward_kernel<true, kMaps, kBucket>, LS::kBytes, configured_t));
   if (kBucket) {
-    GK_TRY(run_band_ids<LD::kC>(plan_r, nullptr, c.bucket, c.buckets, c.n_dst, pitch, ids, st));
-    GK_TRY(run_band_ids<LS::kC>(plan_t, plan_t->eid, c.bucket, c.buckets, c.n_src, pitch_t, ids_t, st));
+    const BandIds other = band_ids_of(plan_t, plan_t->eid, c.n_src, LS::kC, ids_t);
+    GK_TRY(run_band_ids(band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, ids), &other, c.bucket, c.buckets, st));
   }
   t.table = c.table; t.lam = c.lam; t.ids = ids; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan_r->node_lo;
   t.node_deg = plan_r->node_deg; t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.sums = sums; t.d_o = dout;
@@ -999,10 +1028,10 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   if (kBucket) {
     const int smem = c.buckets * threads * (int)sizeof(float);
     GK_TRY(allow_smem(band_bucket_sum_kernel, 56 * 1024, configured_sum));
-    band_bucket_sum_kernel<<<dim3((unsigned)blocks, (unsigned)columns), threads, smem, st>>>(ids, t.g, pieces, c.buckets, columns, partial);
+    band_bucket_sum_kernel<<<dim3((unsigned)blocks, (unsigned)columns), threads, smem, st>>>(ids, t.g, pieces * 32, c.buckets, columns, partial);
     GK_LAUNCHED("band_bucket_sum");
     const int cells = c.buckets * columns;
-    bucket_total_kernel<__nv_bfloat16><<<(cells + 31) / 32, 256, 0, st>>>(partial, (int)blocks, cells, 1.0, d_table);
+    bucket_total_kernel<__nv_bfloat16><<<(cells + 7) / 8, 256, 0, st>>>(partial, (int)blocks, cells, 1.0, d_table);
     GK_LAUNCHED("bucket_total");
   }
   if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, t.t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));

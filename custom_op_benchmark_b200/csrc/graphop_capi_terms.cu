@@ -14,8 +14,6 @@ extern "C" size_t graphop_terms_workspace_bytes(int op, int64_t n_edges, int64_t
     case GRAPHOP_TERMS_DIFF_FWD:
     case GRAPHOP_TERMS_DIFF_BWD:
       return terms_bytes(true, op == GRAPHOP_TERMS_DIFF_BWD, n_edges, n_nodes, H, D, n_buckets, elem_bytes, index_bytes);
-    case GRAPHOP_TERMS_RELATIVE:
-      return graph_bytes(n_edges, n_nodes, index_bytes) + kAlign;
     default:
       return 0;
   }
@@ -24,17 +22,14 @@ extern "C" size_t graphop_terms_workspace_bytes(int op, int64_t n_edges, int64_t
 #define GRAPHOP_DEFINE_RELATIVE(SUF, I)                                                                                              \
   extern "C" int graphop_relative_buckets_##SUF(const I* row, const I* indptr, const I* indices, int64_t n_chunks, const I* dst_pos, \
                                                 const I* src_pos, const int64_t* limits, int n_limits, int both, int32_t* bucket,    \
-                                                int64_t n_edges, void* ws, size_t wsb, graphop_stream_t stream) {                    \
-    if (n_edges > 0) GK_TRY(gk::check_ws(ws));                                                                                       \
-    return gk::relative_buckets<I>(gk::FromChunks<I>{row, indptr, nullptr, indices, (long long)n_chunks, (long long)n_edges},        \
-                                   n_chunks, n_edges, dst_pos, src_pos, limits, n_limits, both, bucket, ws, wsb,                     \
-                                   (cudaStream_t)stream);                                                                            \
+                                                int64_t n_edges, graphop_stream_t stream) {                                          \
+    return gk::relative_chunks<I>(row, indptr, indices, n_chunks, n_edges, dst_pos, src_pos, limits, n_limits, both, bucket,         \
+                                  (cudaStream_t)stream);                                                                             \
   }                                                                                                                                  \
   extern "C" int graphop_relative_buckets_planned_##SUF(const graphop_plan_t* plan, const I* dst_pos, const I* src_pos,              \
                                                         const int64_t* limits, int n_limits, int both, int32_t* bucket,              \
                                                         graphop_stream_t stream) {                                                   \
-    return gk::relative_buckets<I>(gk::FromPlan{plan}, plan ? plan->n_chunks : -1, plan ? plan->n_edges : -1, dst_pos, src_pos,      \
-                                   limits, n_limits, both, bucket, nullptr, 0, (cudaStream_t)stream);                                \
+    return gk::relative_planned<I>(plan, dst_pos, src_pos, limits, n_limits, both, bucket, (cudaStream_t)stream);                    \
   }
 GRAPHOP_DEFINE_RELATIVE(i32, int32_t)
 GRAPHOP_DEFINE_RELATIVE(i64, int64_t)

@@ -700,6 +700,9 @@ def attention_backward_planned(plan_r, plan_t, q, k, v, o, lse, d_o, scale):
 
 # ------------------------------------------------------------------------------------------
 # attention with learned score terms (additions): a bias by buckets, differential attention
+#
+# The forward calls and relative_buckets run in native code (csrc/binding/graphop_native.cpp): in a decoding step their checks and
+# ctypes calls took as long as the kernels.  The code below is for a package built without the compiled modules.
 # ------------------------------------------------------------------------------------------
 def bucket_limits(num_buckets, max_distance):
     """The distances at which the buckets of one direction begin, but for the first: bucket b holds the distances that
@@ -728,7 +731,7 @@ def _limits(num_buckets, max_distance, bidirectional):
     if bidirectional and num_buckets % 2:
         raise ValueError("num_buckets must be even for both directions")
     at = _limits_of(int(num_buckets) // 2 if bidirectional else int(num_buckets), int(max_distance))
-    return (ctypes.c_int64 * len(at))(*at), len(at)
+    return at, (ctypes.c_int64 * len(at))(*at)
 
 
 @functools.lru_cache(maxsize=64)
@@ -759,31 +762,34 @@ def relative_buckets(row, indptr, indices, num_buckets, max_distance, bidirectio
     without it all are for positions behind, and those ahead share bucket 0.  Within a direction the distances are
     shared out as ``bucket_limits`` says.  ``dst_pos`` and ``src_pos`` (index type) default to the node ids; every
     node that an edge names needs a position."""
+    at, limits = _limits(num_buckets, max_distance, bidirectional)
+    native = native_functions_if_built()
+    if native is not None:
+        return native.relative_buckets(row, indptr, indices, at, bool(bidirectional), dst_pos, src_pos)
     _check_all(row=row, indptr=indptr, indices=indices)
     index = _index(row, indptr, indices)
     e, c = indices.size(0), _chunks(row, indptr)
     _positions(dst_pos, src_pos, None, None, indices.dtype, indices.device)
-    limits, n = _limits(num_buckets, max_distance, bidirectional)
     out = th.empty(e, dtype=th.int32, device=indices.device)
-    lib = _capi.lib()
     with th.cuda.device(out.device):
-        _ws, base, need = _scratch(lib.graphop_terms_workspace_bytes(_capi.TERMS_RELATIVE, e, 0, 1, 1, 0, 4, index[1]),
-                                   out.device)
-        _check(getattr(lib, "graphop_relative_buckets_" + index[0])(
-            _owners(row, indptr), _p(indptr), _p(indices), c, _p(dst_pos), _p(src_pos), limits, n, int(bool(bidirectional)), _p(out), e, base,
-            need, th.cuda.current_stream(out.device).cuda_stream), "relative_buckets")
+        _check(getattr(_capi.lib(), "graphop_relative_buckets_" + index[0])(
+            _owners(row, indptr), _p(indptr), _p(indices), c, _p(dst_pos), _p(src_pos), limits, len(at), int(bool(bidirectional)), _p(out), e,
+            th.cuda.current_stream(out.device).cuda_stream), "relative_buckets")
     return out
 
 
 def relative_buckets_planned(plan, num_buckets, max_distance, bidirectional=True, dst_pos=None, src_pos=None):
     """relative_buckets on a plan of the row CSR; the positions are int32 or int64, both the same."""
+    at, limits = _limits(num_buckets, max_distance, bidirectional)
+    native = native_functions_if_built()
+    if native is not None:
+        return native.relative_buckets_planned(plan.native(), at, bool(bidirectional), dst_pos, src_pos, plan._memory)
     dtype = _positions(dst_pos, src_pos, plan.n_nodes, None, None, plan.device)
-    limits, n = _limits(num_buckets, max_distance, bidirectional)
     out = th.empty(plan.n_edges, dtype=th.int32, device=plan.device)
     suffix = "i64" if dtype == th.int64 else "i32"
     with th.cuda.device(out.device):
         _check(getattr(_capi.lib(), "graphop_relative_buckets_planned_" + suffix)(
-            plan.ref(), _p(dst_pos), _p(src_pos), limits, n, int(bool(bidirectional)), _p(out),
+            plan.ref(), _p(dst_pos), _p(src_pos), limits, len(at), int(bool(bidirectional)), _p(out),
             th.cuda.current_stream(out.device).cuda_stream), "relative_buckets_planned")
     return out
 
@@ -922,6 +928,9 @@ def attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale
     A position takes no part where its bucket is outside 0 .. buckets - 1 (-1 marks padding) or its entry of the table is at
     most -1e38 (-inf, a type's lowest value), whatever its rows hold.  A node of which nothing takes part has o = 0,
     lse = -inf.  One destination per sequence and its cached rows as sources, in any order, make a decoding step."""
+    native = native_functions_if_built()
+    if native is not None:
+        return native.attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale)
     graph, e = _rows_graph(row, indptr, indices)
     return _bucket_forward(graph, e, q, k, v, bucket, table, scale)
 
@@ -935,6 +944,9 @@ def attention_bucket_backward(row, indptr, indices, col, indptr_t, eid_t, indice
 
 def attention_bucket_forward_planned(plan, q, k, v, bucket, table, scale):
     """attention_bucket_forward on a plan of the row CSR."""
+    native = native_functions_if_built()
+    if native is not None:
+        return native.attention_bucket_forward_planned(plan.native(), q, k, v, bucket, table, scale)
     graph, e = _plan_rows(plan, q.size(0))
     return _bucket_forward(graph, e, q, k, v, bucket, table, scale)
 
@@ -986,6 +998,9 @@ def attention_diff_forward(row, indptr, indices, q, k, v, lam, scale, bucket=Non
     ``lam`` (h,), of the same type; o (n, h, 2d), lse (n, 2h).  ``parts`` (n, h, 2, 2d), o1 and o2, is what the backward
     reads (None without ``keep_parts``, for a call that has none).  ``bucket`` and ``table`` (buckets, 2h), both or neither: the
     bias of attention_bucket_forward, a column per map, with the same rule for positions that take no part."""
+    native = native_functions_if_built()
+    if native is not None:
+        return native.attention_diff_forward(row, indptr, indices, q, k, v, lam, scale, bucket, table, keep_parts)
     graph, e = _rows_graph(row, indptr, indices)
     return _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts)
 
@@ -999,6 +1014,9 @@ def attention_diff_backward(row, indptr, indices, col, indptr_t, eid_t, indices_
 
 def attention_diff_forward_planned(plan, q, k, v, lam, scale, bucket=None, table=None, keep_parts=True):
     """attention_diff_forward on a plan of the row CSR."""
+    native = native_functions_if_built()
+    if native is not None:
+        return native.attention_diff_forward_planned(plan.native(), q, k, v, lam, scale, bucket, table, keep_parts)
     graph, e = _plan_rows(plan, q.size(0))
     return _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts)
 

@@ -34,11 +34,10 @@ extern "C" {
 #endif
 
 enum {
-  GRAPHOP_TERMS_BUCKET_FWD = 0, GRAPHOP_TERMS_BUCKET_BWD = 1, GRAPHOP_TERMS_DIFF_FWD = 2, GRAPHOP_TERMS_DIFF_BWD = 3,
-  GRAPHOP_TERMS_RELATIVE = 4
+  GRAPHOP_TERMS_BUCKET_FWD = 0, GRAPHOP_TERMS_BUCKET_BWD = 1, GRAPHOP_TERMS_DIFF_FWD = 2, GRAPHOP_TERMS_DIFF_BWD = 3
 };
 
-/* Bytes of workspace of one call.  n_nodes: the larger of n_dst and n_src (any value for RELATIVE); H, D, n_buckets as in the call. */
+/* Bytes of workspace of one call.  n_nodes: the larger of n_dst and n_src; H, D, n_buckets as in the call. */
 size_t graphop_terms_workspace_bytes(int op, int64_t n_edges, int64_t n_nodes, int H, int D, int n_buckets, int elem_bytes,
                                      int index_bytes);
 
@@ -101,10 +100,10 @@ GRAPHOP_DECLARE_TERMS_PLANNED(bf16, uint16_t)
  */
 int graphop_relative_buckets_i32(const int32_t* row, const int32_t* indptr, const int32_t* indices, int64_t n_chunks,
                                  const int32_t* dst_pos, const int32_t* src_pos, const int64_t* limits, int n_limits, int both,
-                                 int32_t* bucket, int64_t n_edges, void* workspace, size_t workspace_bytes, graphop_stream_t stream);
+                                 int32_t* bucket, int64_t n_edges, graphop_stream_t stream);
 int graphop_relative_buckets_i64(const int64_t* row, const int64_t* indptr, const int64_t* indices, int64_t n_chunks,
                                  const int64_t* dst_pos, const int64_t* src_pos, const int64_t* limits, int n_limits, int both,
-                                 int32_t* bucket, int64_t n_edges, void* workspace, size_t workspace_bytes, graphop_stream_t stream);
+                                 int32_t* bucket, int64_t n_edges, graphop_stream_t stream);
 int graphop_relative_buckets_planned_i32(const graphop_plan_t* plan, const int32_t* dst_pos, const int32_t* src_pos,
                                          const int64_t* limits, int n_limits, int both, int32_t* bucket, graphop_stream_t stream);
 int graphop_relative_buckets_planned_i64(const graphop_plan_t* plan, const int64_t* dst_pos, const int64_t* src_pos,

@@ -126,9 +126,9 @@ def test_a_c_program_compiles_against_the_header(tmp_path):
 
 def test_workspace_grows_with_what_it_holds():
     size = _capi.lib().graphop_terms_workspace_bytes
-    for op in range(5):
+    for op in range(4):
         assert 0 < size(op, 1000, 100, 4, 32, 8, 4, 4) < size(op, 100_000, 100, 4, 32, 8, 4, 4) < size(op, 100_000, 100, 4, 32, 8, 4, 8)
-    assert size(5, 1000, 100, 4, 32, 8, 4, 4) == 0 and size(0, -1, 100, 4, 32, 8, 4, 4) == 0
+    assert size(4, 1000, 100, 4, 32, 8, 4, 4) == 0 and size(0, -1, 100, 4, 32, 8, 4, 4) == 0
     assert size(1, 1000, 100, 4, 32, 16385, 4, 4) == 0
     # the pairs of every edge and map
     assert size(_capi.TERMS_DIFF_BWD, 100_000, 100, 4, 32, 0, 4, 4) > 100_000 * 8 * 8
@@ -168,8 +168,8 @@ def test_entry_points_refuse_each_their_own():
     assert _forward_code(nb=0) == [_capi.ERR_WORKSPACE, _capi.ERR_INVALID_ARGUMENT]       # the bias is the differential layer's option
     lib = _capi.lib()
     zeros = (ctypes.c_int64 * 3)(5, 4, 9)
-    assert lib.graphop_relative_buckets_i32(4096, 4096, 4096, 1, None, None, zeros, 3, 1, 4096, 4, 4096, 0, None) == _capi.ERR_INVALID_ARGUMENT
-    assert lib.graphop_relative_buckets_i32(4096, 4096, 4096, 1, None, None, zeros, 1024, 1, 4096, 4, 4096, 0, None) == _capi.ERR_UNSUPPORTED
+    assert lib.graphop_relative_buckets_i32(4096, 4096, 4096, 1, None, None, zeros, 3, 1, 4096, 4, None) == _capi.ERR_INVALID_ARGUMENT
+    assert lib.graphop_relative_buckets_i32(4096, 4096, 4096, 1, None, None, zeros, 1024, 1, 4096, 4, None) == _capi.ERR_UNSUPPORTED
     assert lib.graphop_relative_buckets_planned_i32(None, None, None, zeros, 1, 1, 4096, None) == _capi.ERR_INVALID_ARGUMENT
 
 
