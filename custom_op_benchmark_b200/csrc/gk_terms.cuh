@@ -529,7 +529,7 @@ struct BucketSum {
   int col_stride, columns;    // columns (heads) of x
   int buckets, per, streams, lanes;   // per: columns of a block (blockIdx.y counts such blocks)
 };
-constexpr int kBatch = 8;
+constexpr int kBatch = 16;
 template <typename A>
 __global__ void __launch_bounds__(256)
 bucket_sum_kernel(const A* __restrict__ x, const BucketSum a, double* __restrict__ partial) {
@@ -617,8 +617,11 @@ inline BucketShape bucket_shape(long long rows, int columns, int buckets, int ac
   s.streams = 256 / s.lanes;
   if (s.streams > fit) s.streams = fit < 1 ? 1 : (int)fit;
   s.col_blocks = (columns + s.per - 1) / s.per;
-  // a stream has two batches at least, and the chip four blocks per SM at most, over all blocks of columns: their tables are added up
-  const long long want = rows / (2ll * kBatch * s.streams) + 1, most = 4 * 148 / s.col_blocks + 1;
+  // a stream has two batches at least, and the chip as many blocks as its SMs hold, over all blocks of columns: their tables are added up
+  int per_sm = (int)(200 * 1024 / (s.streams * table + 1024)), threads = s.streams * s.lanes;
+  per_sm = per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm;
+  if (per_sm * threads > 1024) per_sm = 1024 / threads;
+  const long long want = rows / (2ll * kBatch * s.streams) + 1, most = per_sm * 148 / s.col_blocks + 1;
   s.blocks = (int)(want < most ? want : most);
   return s;
 }

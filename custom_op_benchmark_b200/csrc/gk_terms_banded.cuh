@@ -22,7 +22,7 @@
 namespace gk {
 namespace banded {
 
-constexpr int kNoPart = 255;                 // id of an element that takes no part
+constexpr unsigned kNoPart = 255;                 // id of an element that takes no part
 constexpr int kMostBandBuckets = 255;
 
 struct TermsTile {
@@ -39,17 +39,12 @@ struct TermsTile {
   __nv_bfloat16 *o, *parts;
   float* lse;
   // backward
-  const __nv_bfloat16 *sums, *d_o;           // o of every map (n, H, maps, 64); destination side
-  const float* lse_in;
-  float2* stat;                              // (n, H, maps): (lse in base-2 units, dO . o), destination side to source side
-  float* t2;                                 // (n, H): dO . o2
+  float2* stat;                              // (n_dst, H, maps): (lse in base-2 units, dO . o)
   __nv_bfloat16* g;                          // (H, maps, tiles, pitch / 32, 128, 32): score gradients
   __nv_bfloat16 *out0, *out1;                // dq | dk, dv
 };
 
-// first and last column a tile's band reaches, for the whole block: kmin = INT_MAX where no node has a neighbour
-struct BandOf { int lo, deg, kmin, ktop; };
-template <int kWarpsOfRows>
+// first and last column that a warp's 32 rows of a tile reach: INT_MAX and -1 where none has a neighbour
 __device__ __forceinline__ void band_reduce(int lo, int deg, int part, bool writes, int* s_min, int* s_top) {
   int wmin = lo, wtop = deg > 0 ? lo + deg - 1 : -1;
 #pragma unroll
@@ -68,55 +63,64 @@ struct BandIds {
   int pitch, per;        // per: kC
   unsigned char* ids;
 };
-// A warp per row, 32 columns at a time, one per lane: neighbouring positions in one load, and the loads of all of them at once.
-// Bound by the chain node - position - (edge id -) bucket, which every warp goes through once.
+// A warp per row, four columns per lane at a time.  Bound by its instructions (a select per element) and by the chain node - position
+// - (edge id -) bucket, which every warp goes through once; with one column per lane and step, 443 instructions per row, 4.2M edges
+// took 13 us.
 static __global__ void __launch_bounds__(256)
 band_ids_kernel(const __grid_constant__ BandIds a0, const __grid_constant__ BandIds a1, const int32_t* __restrict__ bucket, int buckets) {
-  const BandIds& a = blockIdx.z ? a1 : a0;
+  const bool other = blockIdx.z != 0;
+  const int32_t *node_lo = other ? a1.node_lo : a0.node_lo, *node_deg = other ? a1.node_deg : a0.node_deg,
+                *node_first = other ? a1.node_first : a0.node_first, *eid = other ? a1.eid : a0.eid;
+  const long long n = other ? a1.n : a0.n;
+  const int pitch = other ? a1.pitch : a0.pitch, shift = (other ? a1.per : a0.per) == 32 ? 5 : 4;
   __shared__ int s_min[4], s_top[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long r0 = (long long)blockIdx.x * kTileM;
-  if (r0 >= a.n) return;
+  if (r0 >= n) return;
   const int row = blockIdx.y * 8 + warp;
   const long long r = r0 + row;
   int deg = 0, lo = 0, first = 0;
-  if (r < a.n) {
-    deg = a.node_deg[r];
-    lo = a.node_lo[r];
-    first = a.node_first[r];
+  if (r < n) {
+    deg = node_deg[r];
+    lo = node_lo[r];
+    first = node_first[r];
   }
   if (warp < 4) {
     int l = INT_MAX, d = 0;
-    if (r0 + tid < a.n) {
-      d = a.node_deg[r0 + tid];
-      l = d > 0 ? a.node_lo[r0 + tid] : INT_MAX;
+    if (r0 + tid < n) {
+      d = node_deg[r0 + tid];
+      l = d > 0 ? node_lo[r0 + tid] : INT_MAX;
     }
-    band_reduce<4>(l, d, warp, lane == 0, s_min, s_top);
+    band_reduce(l, d, warp, lane == 0, s_min, s_top);
   }
   __syncthreads();
   const int kmin = min(min(s_min[0], s_min[1]), min(s_min[2], s_min[3]));
-  unsigned char* out = a.ids + (size_t)blockIdx.x * a.pitch * kTileM;
-  const int jlo = deg > 0 ? lo - kmin : 0;
-  constexpr int kSteps = kSpan / 32;
-  int at[kSteps], b[kSteps];
+  unsigned char* out = (other ? a1.ids : a0.ids) + (size_t)blockIdx.x * pitch * kTileM + (row << shift);
+  const int skip = deg > 0 ? lo - kmin : 0;              // columns before the row's first
+  const int32_t* src = eid ? eid : bucket;
+  constexpr int kSteps = kSpan / 128;
+  int b[kSteps][4];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int k = i * 32 + lane - jlo;
-    at[i] = k >= 0 && k < deg ? first + k : -1;
+    const int k = i * 128 + lane * 4 - skip;
+    const int32_t* at = src + ((long long)first + k);    // read where the column is one of the row's alone
+#pragma unroll
+    for (int q = 0; q < 4; ++q) b[i][q] = (unsigned)(k + q) < (unsigned)deg ? __ldg(at + q) : -1;
   }
-  if (a.eid) {
+  if (eid) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
-      if (at[i] >= 0) at[i] = __ldg(a.eid + at[i]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (b[i][q] >= 0) b[i][q] = __ldg(bucket + b[i][q]);
   }
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) b[i] = at[i] >= 0 ? __ldg(bucket + at[i]) : -1;
-  const int shift = a.per == 32 ? 5 : 4;
-#pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int c = i * 32 + lane;
-    if (c < a.pitch)
-      out[(((size_t)(c >> shift) * kTileM + row) << shift) + (c & (a.per - 1))] = (unsigned)b[i] < (unsigned)buckets ? b[i] : kNoPart;
+    const int c = i * 128 + lane * 4;
+    unsigned w = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w |= ((unsigned)b[i][q] < (unsigned)buckets ? (unsigned)b[i][q] : kNoPart) << (8 * q);
+    if (c < pitch) *reinterpret_cast<unsigned*>(out + ((size_t)(c >> shift) << (shift + 7)) + (c & ((1 << shift) - 1))) = w;
   }
 }
 
@@ -228,7 +232,7 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     deg = p.node_deg[r];
     if (deg > 0) lo = p.node_lo[r];
   }
-  band_reduce<4>(lo, deg, quarter, lane == 0 && cg == 0, s_min, s_top);
+  band_reduce(lo, deg, quarter, lane == 0 && cg == 0, s_min, s_top);
   fill_table<kBucket>(s_table, p, kMaps, head, tid);
   if (tid == 0) {
     mbar_init(bar_load, 1);
@@ -454,7 +458,7 @@ struct BwdLayout {
   static constexpr int kOffStage = kOffC + kSlots * kSlot;
   static constexpr int kOffBar = kOffStage + kStages * kBlockBytes;
   static constexpr int kOffStat = kOffBar + 128;
-  static constexpr int kStatBytes = kSrc ? kSpan * kMaps * 8 : kMaps * kColGroups * kTileM * 4;
+  static constexpr int kStatBytes = kSrc ? kSpan * kMaps * 8 : 0;
   static constexpr int kOffTable = kOffStat + kStatBytes;
   static constexpr int kBytes = kOffTable + kMaps * 256 * 4 + 1024;
   // tensor memory: scores of every map, dP, then dq | dk, dv
@@ -463,10 +467,8 @@ struct BwdLayout {
 };
 
 template <bool kSrc, int kMaps, bool kBucket>
-__global__ void __launch_bounds__(kThreads, 2)
-terms_backward_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                      const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_d,
-                      const __grid_constant__ TermsTile p) {
+__device__ __forceinline__ void terms_backward_tile(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_c,
+                                                    const CUtensorMap& map_d, const TermsTile& p, unsigned tiles) {
   using L = BwdLayout<kSrc, kMaps>;
   constexpr int kB = L::kB, kC = L::kC;
   extern __shared__ unsigned char raw_smem[];
@@ -477,7 +479,6 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   int* s_min = reinterpret_cast<int*>(smem + L::kOffBar + 40);
   int* s_top = reinterpret_cast<int*>(smem + L::kOffBar + 96);
   float2* s_stat = reinterpret_cast<float2*>(smem + L::kOffStat);   // source side: [query][map]
-  float* s_part = reinterpret_cast<float*>(smem + L::kOffStat);     // destination side: [map][column group][row] parts of dO . o
   float* s_table = reinterpret_cast<float*>(smem + L::kOffTable);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -489,7 +490,7 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     deg = p.node_deg[r];
     if (deg > 0) lo = p.node_lo[r];
   }
-  band_reduce<4>(lo, deg, quarter, lane == 0 && cg == 0, s_min, s_top);
+  band_reduce(lo, deg, quarter, lane == 0 && cg == 0, s_min, s_top);
   fill_table<kBucket>(s_table, p, kMaps, head, tid);
   if (tid == 0) {
     mbar_init(bar_load, 1);
@@ -532,56 +533,21 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       if (nb > 1) issue_band(1);
     }
     int issued = nb < kSlots ? nb : kSlots;
-    // per-row scalars while the tiles travel
+    // the rows' statistics while the tiles travel; column j of the source side's scores is query bmin + j
     float lse2[kMaps], delta[kMaps];
 #pragma unroll
-    for (int m = 0; m < kMaps; ++m) lse2[m] = delta[m] = 0.f;
-    if constexpr (!kSrc) {
-      // dO . o of the row's maps: each of its two threads takes 32 of the 64 features
-      float part[kMaps];
-#pragma unroll
-      for (int m = 0; m < kMaps; ++m) part[m] = 0.f;
-      if (r < p.n_own) {
-        const uint4* grow = reinterpret_cast<const uint4*>(p.d_o + ((long long)r * p.H + head) * kD) + cg * 4;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint4 gv = __ldg(grow + q);
-          const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv);
-#pragma unroll
-          for (int m = 0; m < kMaps; ++m) {
-            const uint4 ov = __ldg(reinterpret_cast<const uint4*>(p.sums + (cell + m) * kD) + cg * 4 + q);
-            const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&ov);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 of = __bfloat1622float2(o2[e]), gf = __bfloat1622float2(g2[e]);
-              part[m] += of.x * gf.x + of.y * gf.y;
-            }
-          }
-        }
-#pragma unroll
-        for (int m = 0; m < kMaps; ++m) lse2[m] = p.lse_in[cell + m];
-      }
-#pragma unroll
-      for (int m = 0; m < kMaps; ++m) s_part[(m * kColGroups + cg) * kTileM + row] = part[m];
-    } else {
-      // the statistics of the band's queries: column j of the scores is query bmin + j
+    for (int m = 0; m < kMaps; ++m) {
+      const float2 st = !kSrc && r < p.n_own ? p.stat[cell + m] : make_float2(INFINITY, 0.f);
+      lse2[m] = st.x;
+      delta[m] = st.y;
+    }
+    if constexpr (kSrc) {
       for (int i = tid; i < nb * kB * kMaps; i += kThreads) {
         const long long qn = (long long)bmin + i / kMaps;
         s_stat[i] = qn < p.n_other ? p.stat[(qn * p.H + head) * kMaps + i % kMaps] : make_float2(INFINITY, 0.f);
       }
     }
     ok = __syncthreads_and(mbar_wait(bar_load, 0) && mbar_wait(bar_full, 0));
-    if constexpr (!kSrc) {
-#pragma unroll
-      for (int m = 0; m < kMaps; ++m) {
-        // the same order in both threads; a row of which nothing took part has no probabilities, whatever dO holds
-        const bool none = lse2[m] == -INFINITY;
-        delta[m] = none ? 0.f : s_part[(m * kColGroups) * kTileM + row] + s_part[(m * kColGroups + 1) * kTileM + row];
-        lse2[m] = none ? INFINITY : lse2[m] * (float)kLog2e;
-        if (cg == 0 && r < p.n_own) p.stat[cell + m] = make_float2(lse2[m], delta[m]);
-      }
-      if (kMaps == 2 && cg == 0 && r < p.n_own) p.t2[(long long)r * p.H + head] = delta[kMaps - 1];
-    }
 
     const int jlo = deg > 0 ? lo - bmin : 1, jhi = deg > 0 ? lo - bmin + deg - 1 : 0;
     int wlo = deg > 0 ? jlo : INT_MAX, whi = deg > 0 ? jhi : -1;
@@ -665,7 +631,7 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
           if constexpr (kBucket && !kSrc) {
 #pragma unroll
             for (int m = 0; m < kMaps; ++m) {
-              uint4* at = reinterpret_cast<uint4*>(p.g + ((size_t)(head * kMaps + m) * gridDim.x * p.pitch * kTileM + tile_at +
+              uint4* at = reinterpret_cast<uint4*>(p.g + ((size_t)(head * kMaps + m) * tiles * p.pitch * kTileM + tile_at +
                                                          (size_t)(2 * b + cg) * kC * kTileM + row * kC + half * 16));
               at[0] = make_uint4(pg[m][0], pg[m][1], pg[m][2], pg[m][3]);
               at[1] = make_uint4(pg[m][4], pg[m][5], pg[m][6], pg[m][7]);
@@ -741,19 +707,71 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       *reinterpret_cast<uint4*>(p.out0 + at + q * 8) = make_uint4(0, 0, 0, 0);
       if constexpr (kSrc) *reinterpret_cast<uint4*>(p.out1 + at + q * 8) = make_uint4(0, 0, 0, 0);
     }
-    if constexpr (!kSrc) {
-#pragma unroll
-      for (int m = 0; m < kMaps; ++m) p.stat[cell + m] = make_float2(INFINITY, 0.f);
-      if (kMaps == 2) p.t2[(long long)r * p.H + head] = 0.f;
-    }
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   bad = __syncthreads_or(bad);
-  if (tid == 0) p.dirty[(size_t)head * gridDim.x + blockIdx.x] = bad;
+  if (tid == 0) p.dirty[(size_t)head * tiles + blockIdx.x] = bad;
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmem) : "memory");
 }
+
+// Both sides in one launch, the destination's tiles first: 1024 tiles two to an SM are 3.5 rounds of the chip, which take the time of
+// four; twice as many are seven (2 x 8192 nodes, 8 heads: 78 + 82 us apart).
+template <int kMaps, bool kBucket>
+__global__ void __launch_bounds__(kThreads, 2)
+terms_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
+                      const __grid_constant__ CUtensorMap band_q, const __grid_constant__ CUtensorMap band_g,
+                      const __grid_constant__ TermsTile dst, const __grid_constant__ TermsTile src, const unsigned tiles_dst,
+                      const unsigned tiles_src) {
+  if (blockIdx.z == 0) {
+    if (blockIdx.x < tiles_dst) terms_backward_tile<false, kMaps, kBucket>(map_q, map_g, map_k, map_v, dst, tiles_dst);
+  } else {
+    if (blockIdx.x < tiles_src) terms_backward_tile<true, kMaps, kBucket>(map_k, map_v, band_q, band_g, src, tiles_src);
+  }
+}
+
+// What the tiles' rows need: (lse in base-2 units, dO . o) of every node and map, and dO . o2 for dlam.  Eight lanes per node and head.
+// A row of which nothing took part has no probabilities, whatever dO holds.
+template <int kMaps>
+__global__ void __launch_bounds__(256)
+band_stat_kernel(const __nv_bfloat16* __restrict__ sums, const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse, long long cells,
+                 float2* __restrict__ stat, float* __restrict__ t2) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
+  const int part = threadIdx.x & 7;
+  const bool in = i < cells;
+  float d[kMaps];
+#pragma unroll
+  for (int m = 0; m < kMaps; ++m) d[m] = 0.f;
+  if (in) {
+    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(d_o + i * kD) + part);
+    const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv);
+#pragma unroll
+    for (int m = 0; m < kMaps; ++m) {
+      const uint4 ov = __ldg(reinterpret_cast<const uint4*>(sums + (i * kMaps + m) * kD) + part);
+      const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&ov);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 of = __bfloat1622float2(o2[e]), gf = __bfloat1622float2(g2[e]);
+        d[m] += of.x * gf.x + of.y * gf.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kMaps; ++m) {
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) d[m] += __shfl_xor_sync(kFull, d[m], o);
+    if (in && part == 0) {
+      const float l = lse[i * kMaps + m];
+      const bool none = l == -INFINITY;
+      if (none) d[m] = 0.f;
+      stat[i * kMaps + m] = make_float2(none ? INFINITY : l * (float)kLog2e, d[m]);
+      if (m == 1) t2[i] = d[m];
+    }
+  }
+}
+
 
 // ---------------------------------------------------------------------------------------------------------
 // tiles done again, edge by edge: kSide 0 forward, 1 destination side (dq), 2 source side (dk, dv)
@@ -863,47 +881,82 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
 // dT: sums of g by bucket, over the tiles' elements in the threads' order
 // ---------------------------------------------------------------------------------------------------------
 // grid: (blocks, H * maps).  A thread takes 8 elements at a time, so that a warp's loads are whole lines, and asks for kAhead such
-// pieces at once; they go into a table of its own, cell b of thread t at b * blockDim.x + t: a warp's 32 cells lie in 32 banks.
-// Bound by reading the gradients and, once per head, the ids.
-static __global__ void __launch_bounds__(128)
+// pieces at once; they go into a table of its own, cell b of thread t at b * NT + t: a warp's 32 cells lie in 32 banks.  An element
+// that takes no part has a gradient of zero and goes to one cell more.  Bound by its instructions, about ten per element (with a test
+// per element and the table's stride not known, 14: 36 us for 6.3M elements of 8 heads), then by reading the gradients.
+template <int NT>
+__global__ void __launch_bounds__(NT)
 band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const __nv_bfloat16* __restrict__ g, long long elements, int buckets,
                        int columns, double* __restrict__ partial) {
   extern __shared__ float cells[];
   constexpr int kAhead = 4;
-  const int tid = threadIdx.x, nt = blockDim.x, column = blockIdx.y;
-  const long long pieces = elements / 8, stride = (long long)gridDim.x * nt;
+  const int tid = threadIdx.x, column = blockIdx.y;
+  const long long pieces = elements / 8, stride = (long long)gridDim.x * NT;
   const uint2* idp = reinterpret_cast<const uint2*>(ids);
   const uint4* src = reinterpret_cast<const uint4*>(g + (size_t)column * elements);
-  for (int b = 0; b < buckets; ++b) cells[b * nt + tid] = 0.f;
-  for (long long i = (long long)blockIdx.x * nt + tid; i < pieces; i += kAhead * stride) {
+  float* mine = cells + tid;
+  for (int b = 0; b <= buckets; ++b) mine[b * NT] = 0.f;
+  const unsigned none = (unsigned)buckets;
+  for (long long i = (long long)blockIdx.x * NT + tid; i < pieces; i += kAhead * stride) {
     uint2 id[kAhead];
     uint4 w[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) id[k] = i + k * stride < pieces ? __ldg(idp + i + k * stride) : make_uint2(0xffffffffu, 0xffffffffu);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if ((id[k].x & id[k].y) != 0xffffffffu) w[k] = __ldg(src + i + k * stride);   // else nothing takes part
+      if ((id[k].x & id[k].y) != 0xffffffffu) w[k] = __ldg(src + i + k * stride);   // else nothing takes part, and nothing was stored
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if ((id[k].x & id[k].y) == 0xffffffffu) continue;
-      const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w[k]);
+      const unsigned v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const unsigned b = ((j < 4 ? id[k].x : id[k].y) >> (8 * (j & 3))) & 255u;
-        const float v = (j & 1) ? __high2float(x[j >> 1]) : __low2float(x[j >> 1]);
-        if (b < (unsigned)buckets) cells[b * nt + tid] += v;
+        const unsigned b = min(((j < 4 ? id[k].x : id[k].y) >> (8 * (j & 3))) & 255u, none);
+        mine[b * NT] += __uint_as_float((j & 1) ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
       }
     }
   }
   __syncthreads();
   const int warp = tid >> 5, lane = tid & 31;
-  for (int b = warp; b < buckets; b += nt / 32) {   // a bucket per warp: the threads' cells in order, by halves
+  for (int b = warp; b < buckets; b += NT / 32) {   // a bucket per warp: the threads' cells in order, by halves
     double s = 0;
-    for (int t = lane; t < nt; t += 32) s += (double)cells[b * nt + t];
+#pragma unroll
+    for (int t = 0; t < NT; t += 32) s += (double)cells[b * NT + t + lane];
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
     if (lane == 0) partial[((size_t)blockIdx.x * buckets + b) * columns + column] = s;
   }
+}
+// A block has a table per thread; as many blocks as share the SMs' memory, a piece or more for every thread.
+struct BandSumShape { int threads, smem, blocks; };
+inline BandSumShape band_sum_shape(long long elements, int buckets, int columns) {
+  BandSumShape s;
+  s.threads = 128;
+  while (s.threads > 32 && (buckets + 1) * s.threads * (int)sizeof(float) > 56 * 1024) s.threads >>= 1;
+  s.smem = (buckets + 1) * s.threads * (int)sizeof(float);
+  long long per_sm = 200 * 1024 / (s.smem + 1024);
+  per_sm = per_sm > 10 ? 10 : per_sm;
+  long long blocks = per_sm * 148 / columns, most = elements / 8 / s.threads + 1;
+  blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
+  s.blocks = (int)blocks;
+  return s;
+}
+inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, const __nv_bfloat16* g, long long elements, int buckets,
+                               int columns, double* partial, __nv_bfloat16* out, cudaStream_t st) {
+  const auto launch = [&](auto kernel, std::atomic<bool> (&configured)[64]) -> int {
+    GK_TRY(allow_smem(kernel, 56 * 1024, configured));
+    kernel<<<dim3((unsigned)s.blocks, (unsigned)columns), s.threads, s.smem, st>>>(ids, g, elements, buckets, columns, partial);
+    GK_LAUNCHED("band_bucket_sum");
+    return GRAPHOP_OK;
+  };
+  static std::atomic<bool> c128[64], c64[64], c32[64];
+  if (s.threads == 128) GK_TRY(launch(band_bucket_sum_kernel<128>, c128));
+  else if (s.threads == 64) GK_TRY(launch(band_bucket_sum_kernel<64>, c64));
+  else GK_TRY(launch(band_bucket_sum_kernel<32>, c32));
+  const int cells = buckets * columns;
+  bucket_total_kernel<__nv_bfloat16><<<(cells + 7) / 8, 256, 0, st>>>(partial, s.blocks, cells, 1.0, out);
+  GK_LAUNCHED("bucket_total");
+  return GRAPHOP_OK;
 }
 
 // (n, H, 64) bf16 node tensor as make_map's, in boxes of `rows` nodes
@@ -974,14 +1027,8 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   using LD = BwdLayout<false, kMaps>;
   using LS = BwdLayout<true, kMaps>;
   const int pitch = band_pitch(plan_r), pitch_t = band_pitch(plan_t), columns = c.H * kMaps;
-  const long long tiles = band_tiles_of(c.n_dst), tiles_t = band_tiles_of(c.n_src), pieces = tiles * pitch / 32 * kTileM;
-  // dT's sums: a block has a table per thread; as many blocks as share the SMs' memory, a piece or more for every thread
-  int threads = 128;
-  while (threads > 32 && (size_t)c.buckets * threads * sizeof(float) > 56 * 1024) threads >>= 1;
-  long long per_sm = kBucket ? 200 * 1024 / ((long long)c.buckets * threads * (long long)sizeof(float) + 1024) : 1;
-  if (per_sm > 8) per_sm = 8;
-  long long blocks = (per_sm * 148 + columns - 1) / columns;
-  if (blocks > pieces / threads + 1) blocks = pieces / threads + 1;
+  const long long tiles = band_tiles_of(c.n_dst), tiles_t = band_tiles_of(c.n_src), elements = tiles * pitch * kTileM;
+  const BandSumShape sum = kBucket ? band_sum_shape(elements, c.buckets, columns) : BandSumShape{};
 
   TermsTile t{};
   t.stat = (float2*)ar.take((size_t)c.n_dst * columns * sizeof(float2));
@@ -989,12 +1036,12 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   int* dirty_t = (int*)ar.take((size_t)tiles_t * c.H * sizeof(int));
   unsigned char *ids = nullptr, *ids_t = nullptr;
   double* partial = nullptr;
-  if (kMaps == 2) t.t2 = (float*)ar.take((size_t)c.n_dst * c.H * sizeof(float));
+  float* t2 = kMaps == 2 ? (float*)ar.take((size_t)c.n_dst * c.H * sizeof(float)) : nullptr;
   if (kBucket) {
-    ids = (unsigned char*)ar.take((size_t)tiles * pitch * kTileM);
+    ids = (unsigned char*)ar.take((size_t)elements);
     ids_t = (unsigned char*)ar.take((size_t)tiles_t * pitch_t * kTileM);
-    t.g = (__nv_bfloat16*)ar.take((size_t)columns * pieces * 32 * sizeof(__nv_bfloat16));
-    partial = (double*)ar.take((size_t)blocks * c.buckets * columns * sizeof(double));
+    t.g = (__nv_bfloat16*)ar.take((size_t)columns * elements * sizeof(__nv_bfloat16));
+    partial = (double*)ar.take((size_t)sum.blocks * c.buckets * columns * sizeof(double));
   }
   const size_t before_sum = ar.used;
   if (kMaps == 2) ar.take(bucket_sum_bytes(c.n_dst, c.H, 1, 4));
@@ -1005,36 +1052,28 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
       !make_map(&mg, dout, c.n_dst, c.H) || !make_map_rows(&mqs, c.q, c.n_dst, c.H, LS::kB) ||
       !make_map_rows(&mgs, dout, c.n_dst, c.H, LS::kB))
     return GRAPHOP_ERR_UNSUPPORTED;
-  static std::atomic<bool> configured[64], configured_t[64], configured_sum[64];
-  GK_TRY(allow_smem(terms_backward_kernel<false, kMaps, kBucket>, LD::kBytes, configured));
-  GK_TRY(allow_smem(terms_backward_kernel<true, kMaps, kBucket>, LS::kBytes, configured_t));
+  constexpr int smem = LD::kBytes > LS::kBytes ? LD::kBytes : LS::kBytes;
+  static std::atomic<bool> configured[64];
+  GK_TRY(allow_smem(terms_backward_kernel<kMaps, kBucket>, smem, configured));
   if (kBucket) {
     const BandIds other = band_ids_of(plan_t, plan_t->eid, c.n_src, LS::kC, ids_t);
     GK_TRY(run_band_ids(band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, ids), &other, c.bucket, c.buckets, st));
   }
+  const long long cells = c.n_dst * c.H;
+  band_stat_kernel<kMaps><<<(unsigned)((cells * 8 + 255) / 256), 256, 0, st>>>(sums, dout, (const float*)lse, cells, t.stat, t2);
+  GK_LAUNCHED("band_stat");
   t.table = c.table; t.lam = c.lam; t.ids = ids; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan_r->node_lo;
-  t.node_deg = plan_r->node_deg; t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.sums = sums; t.d_o = dout;
-  t.lse_in = (const float*)lse; t.out0 = dq;
-  terms_backward_kernel<false, kMaps, kBucket><<<dim3((unsigned)tiles, (unsigned)c.H), kThreads, LD::kBytes, st>>>(mq, mg, mk, mv, t);
-  GK_LAUNCHED(kMaps == 2 ? "attention_diff_bwd_dst_banded" : "attention_bucket_bwd_dst_banded");
-  AgainArgs a{t, c.q, c.k, c.v, dout, plan_r->node_first, nullptr, c.bucket, (int)tiles};
-  GK_TRY((run_band_again<1, kMaps, kBucket>(a, st)));
-  t.ids = ids_t; t.pitch = pitch_t; t.node_lo = plan_t->node_lo; t.node_deg = plan_t->node_deg; t.dirty = dirty_t; t.n_own = c.n_src;
-  t.n_other = c.n_dst; t.out0 = dk; t.out1 = dv;
-  terms_backward_kernel<true, kMaps, kBucket><<<dim3((unsigned)tiles_t, (unsigned)c.H), kThreads, LS::kBytes, st>>>(mk, mv, mqs, mgs, t);
-  GK_LAUNCHED(kMaps == 2 ? "attention_diff_bwd_src_banded" : "attention_bucket_bwd_src_banded");
-  a = AgainArgs{t, c.q, c.k, c.v, dout, plan_t->node_first, plan_t->eid, c.bucket, (int)tiles_t};
-  GK_TRY((run_band_again<2, kMaps, kBucket>(a, st)));
-  if (kBucket) {
-    const int smem = c.buckets * threads * (int)sizeof(float);
-    GK_TRY(allow_smem(band_bucket_sum_kernel, 56 * 1024, configured_sum));
-    band_bucket_sum_kernel<<<dim3((unsigned)blocks, (unsigned)columns), threads, smem, st>>>(ids, t.g, pieces * 32, c.buckets, columns, partial);
-    GK_LAUNCHED("band_bucket_sum");
-    const int cells = c.buckets * columns;
-    bucket_total_kernel<__nv_bfloat16><<<(cells + 7) / 8, 256, 0, st>>>(partial, (int)blocks, cells, 1.0, d_table);
-    GK_LAUNCHED("bucket_total");
-  }
-  if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, t.t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));
+  t.node_deg = plan_r->node_deg; t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.out0 = dq;
+  TermsTile u = t;
+  u.ids = ids_t; u.pitch = pitch_t; u.node_lo = plan_t->node_lo; u.node_deg = plan_t->node_deg; u.dirty = dirty_t; u.n_own = c.n_src;
+  u.n_other = c.n_dst; u.out0 = dk; u.out1 = dv;
+  terms_backward_kernel<kMaps, kBucket><<<dim3((unsigned)(tiles > tiles_t ? tiles : tiles_t), (unsigned)c.H, 2), kThreads, smem, st>>>(
+      mq, mk, mv, mg, mqs, mgs, t, u, (unsigned)tiles, (unsigned)tiles_t);
+  GK_LAUNCHED(kMaps == 2 ? "attention_diff_bwd_banded" : "attention_bucket_bwd_banded");
+  GK_TRY((run_band_again<1, kMaps, kBucket>(AgainArgs{t, c.q, c.k, c.v, dout, plan_r->node_first, nullptr, c.bucket, (int)tiles}, st)));
+  GK_TRY((run_band_again<2, kMaps, kBucket>(AgainArgs{u, c.q, c.k, c.v, dout, plan_t->node_first, plan_t->eid, c.bucket, (int)tiles_t}, st)));
+  if (kBucket) GK_TRY(run_band_bucket_sum(sum, ids, t.g, elements, c.buckets, columns, partial, d_table, st));
+  if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));
   return GRAPHOP_OK;
 }
 
