@@ -106,7 +106,7 @@ struct TermsBias {
 };
 
 template <class GEO, int kMaps, bool kBucket>
-struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 1 + kMaps, 1, 0, 2> {
+struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 1 + kMaps, 1, 0, 2, (sizeof(typename GEO::T) > 2)> {
   using T = typename GEO::T;
   using A = typename GEO::A;
   using F = typename GEO::F;
@@ -176,15 +176,23 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
         mn[m] = s[v][m] > mn[m] ? s[v][m] : mn[m];
       }
     }
+    // The sums are relative to a reference that may lag behind the maximum by up to 2^8 (the rounding is relative), so that after a
+    // node's first edges they are seldom rescaled.
+    bool grows = false;
 #pragma unroll
-    for (int m = 0; m < kMaps; ++m) {
-      const A corr = st.m[m] == mn[m] ? A(1) : gk_exp2(st.m[m] - mn[m]);   // m = -inf before a node's first edge: 2^-inf = 0
-      ref[m] = mn[m] == neg_inf<A>() ? A(0) : mn[m];                       // nothing has taken part so far: 2^-inf
-      st.m[m] = mn[m];
-      st.l[m] *= corr;
+    for (int m = 0; m < kMaps; ++m) grows = grows || mn[m] > st.m[m] + A(8);   // m = -inf before a node's first edge
+    if (__any_sync(kFull, grows)) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) st.acc[m][i].scale(corr);
+      for (int m = 0; m < kMaps; ++m) {
+        const A corr = st.m[m] == mn[m] ? A(1) : gk_exp2(st.m[m] - mn[m]);
+        st.m[m] = mn[m];
+        st.l[m] *= corr;
+#pragma unroll
+        for (int i = 0; i < W; ++i) st.acc[m][i].scale(corr);
+      }
     }
+#pragma unroll
+    for (int m = 0; m < kMaps; ++m) ref[m] = st.m[m] == neg_inf<A>() ? A(0) : st.m[m];   // nothing has taken part so far: 2^-inf
 #pragma unroll
     for (int v = 0; v < N; ++v) {
       F f[W];
