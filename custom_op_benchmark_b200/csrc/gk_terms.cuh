@@ -105,8 +105,17 @@ struct TermsBias {
   }
 };
 
+// Two maps of 2-byte elements: registers that the maps and the table's addresses take beyond the fragments, in fragments.  R-MAT 16, 8
+// pairs of 64 with a bias, forward 1217 us with none more (108 bytes a thread spill), 1018 with one, 1102 with four (nothing spills, 16
+// warps per SM); 600 thousand edges, 3 pairs of 32, destination side 226 us with none more, 188 with three.
 template <class GEO, int kMaps, bool kBucket>
-struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 1 + kMaps, 1, 0, 2, (sizeof(typename GEO::T) > 2)> {
+constexpr int kTermsMoreFwd = kMaps == 2 && sizeof(typename GEO::T) == 2 ? 1 : 0;
+template <class GEO, int kMaps, bool kBucket>
+constexpr int kTermsMoreDst = kMaps == 2 && kBucket && sizeof(typename GEO::T) == 2 ? 3 : 0;
+
+template <class GEO, int kMaps, bool kBucket>
+struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 1 + kMaps + kTermsMoreFwd<GEO, kMaps, kBucket>, 1, 0, 2,
+                         (sizeof(typename GEO::T) > 2)> {
   using T = typename GEO::T;
   using A = typename GEO::A;
   using F = typename GEO::F;
@@ -299,7 +308,7 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
 
 // Destination side of the backward: dq, the pairs (p1 - lam p2, g) per position and map, t2 per node for dlam.
 template <class GEO, int kMaps, bool kBucket>
-struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 4, 2 + kMaps, kMaps * (int)sizeof(typename GEO::A),
+struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 4 + kTermsMoreDst<GEO, kMaps, kBucket>, 2 + kMaps, kMaps * (int)sizeof(typename GEO::A),
                             (sizeof(typename GEO::T) == 2 ? 2 : 1), true> {
   using T = typename GEO::T;
   using A = typename GEO::A;
