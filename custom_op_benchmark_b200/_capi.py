@@ -93,7 +93,7 @@ UNTYPED = {
 # include/graphop_terms.h: the attention layers with learned score terms
 TERMS_BUCKET_FWD, TERMS_BUCKET_BWD, TERMS_DIFF_FWD, TERMS_DIFF_BWD = range(4)
 TERMS_SIGNATURES = {
-    "attention_bucket_forward": [_P] * 3 + [_I64] + [_P] * 5 + [_INT, _DBL] + [_P] * 2 + [_I64] * 3 + [_INT] * 2 + _TAIL,
+    "attention_bucket_forward": [_P] * 3 + [_I64] + [_P] * 5 + [_INT, _DBL] + [_P] * 3 + [_I64] * 3 + [_INT] * 2 + _TAIL,
     "attention_bucket_backward": [_P] * 3 + [_I64] + [_P] * 4 + [_I64] + [_P] * 5 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 4
                                  + [_I64] * 3 + [_INT] * 2 + _TAIL,
     "attention_diff_forward": [_P] * 3 + [_I64] + [_P] * 6 + [_INT, _DBL] + [_P] * 3 + [_I64] * 3 + [_INT] * 2 + _TAIL,
@@ -101,7 +101,7 @@ TERMS_SIGNATURES = {
                                + [_I64] * 3 + [_INT] * 2 + _TAIL,
 }
 TERMS_PLANNED_SIGNATURES = {
-    "attention_bucket_forward_planned": [_PP] + [_P] * 5 + [_INT, _DBL] + [_P] * 2 + [_I64] * 2 + [_INT] * 2 + _TAIL,
+    "attention_bucket_forward_planned": [_PP] + [_P] * 5 + [_INT, _DBL] + [_P] * 3 + [_I64] * 2 + [_INT] * 2 + _TAIL,
     "attention_bucket_backward_planned": [_PP] * 2 + [_P] * 5 + [_INT] + [_P] * 3 + [_DBL] + [_P] * 4 + [_I64] * 2
                                          + [_INT] * 2 + _TAIL,
     "attention_diff_forward_planned": [_PP] + [_P] * 6 + [_INT, _DBL] + [_P] * 3 + [_I64] * 2 + [_INT] * 2 + _TAIL,

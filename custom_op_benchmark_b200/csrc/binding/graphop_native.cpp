@@ -677,13 +677,13 @@ struct TermsBackward : GraphNode {
   variable_list apply(variable_list&& grads) override {
     const size_t n_grads = diff ? 5 : 4;   // q, k, v (, lam), table
     if (!grads[0].defined()) return variable_list(n_grads);
-    const std::vector<Tensor> t = unpack_saved();   // q, k, v, lam, bucket, table, lse, o or parts (, the seven index tensors)
+    const std::vector<Tensor> t = unpack_saved();   // q, k, v, lam, bucket, table, lse, sums (, the seven index tensors)
     const TermsInputs x{t[0], t[1], t[2], t[3], t[4], t[5]};
     const Tensor &lse = t[6], &o = t[7], g = upstream(grads, "d_o");
     const bool planned = rows != nullptr;
     const int64_t e = planned ? rows->plan.n_edges : t[10].size(0);
     const TermsShape s = check_terms(x, diff, e);
-    elem_of({&x.q, &o, &g});
+    elem_of({&x.q, &g});
     int ib = 4;
     if (!planned) {
       const std::vector<Tensor> index(t.begin() + 8, t.begin() + 15);
@@ -703,8 +703,8 @@ struct TermsBackward : GraphNode {
     // f(graph arguments..., then) with `then` the arguments after the graph's
     const auto typed = [&](auto* y, auto&& call) {
       using E = std::remove_pointer_t<decltype(y)>;
-      const E *q = ptr<E>(x.q), *k = ptr<E>(x.k), *v = ptr<E>(x.v), *lam = ptr<E>(x.lam), *table = ptr<E>(x.table), *out = ptr<E>(o),
-              *up = ptr<E>(g);
+      const E *q = ptr<E>(x.q), *k = ptr<E>(x.k), *v = ptr<E>(x.v), *lam = ptr<E>(x.lam), *table = ptr<E>(x.table), *up = ptr<E>(g);
+      const void* out = o.data_ptr();
       return call(q, k, v, lam, ids(x.bucket), table, s.buckets, out, (const void*)lse.data_ptr(), up, scale, ptr<E>(dq), ptr<E>(dk),
                   ptr<E>(dv), ptr<E>(dl), ptr<E>(dt));
     };
@@ -742,7 +742,7 @@ struct TermsBackward : GraphNode {
   }
 };
 
-// o; lse and parts as the entry point leaves them.  `keep`: parts whether or not a gradient will be asked for.
+// o; lse and the unrounded sums as the entry point leaves them.  `keep`: the sums whether or not a gradient will be asked for.
 struct TermsOutputs { Tensor o, lse, parts; };
 TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool diff, double scale, bool track, bool keep) {
   const int64_t e = graph.edges();
@@ -761,12 +761,15 @@ TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool d
                        x.q.options());
   const int64_t maps = diff ? 2 * s.H : s.H;
   Tensor lse = at::empty({s.n, maps}, x.q.options().dtype(s.elem == 1 ? at::kDouble : at::kFloat)), parts;
-  if (diff && (grads || keep)) parts = at::empty({s.n, s.H, 2, 2 * s.D}, x.q.options());
+  const auto acc = s.elem == 1 ? at::kDouble : at::kFloat;
+  if (diff && (grads || keep)) parts = at::empty({s.n, s.H, 2, 2 * s.D}, x.q.options().dtype(acc));
+  if (!diff && (grads || keep) && x.q.scalar_type() != acc) parts = at::empty(o.sizes(), x.q.options().dtype(acc));   // else o serves
   terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_FWD : GRAPHOP_TERMS_BUCKET_FWD, e, s, x.q, ib);
   const auto typed = [&](auto* y, auto&& call) {
     using E = std::remove_pointer_t<decltype(y)>;
     const E *q = ptr<E>(x.q), *k = ptr<E>(x.k), *v = ptr<E>(x.v), *lam = ptr<E>(x.lam), *table = ptr<E>(x.table);
-    return call(q, k, v, lam, ids(x.bucket), table, s.buckets, scale, ptr<E>(o), ptr<E>(parts), (void*)lse.data_ptr());
+    return call(q, k, v, lam, ids(x.bucket), table, s.buckets, scale, ptr<E>(o), parts.defined() ? parts.data_ptr() : nullptr,
+                (void*)lse.data_ptr());
   };
   int rc;
   if (graph.planned()) {
@@ -775,7 +778,7 @@ TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool d
       return typed(y, [&](auto q, auto k, auto v, auto lam, auto bucket, auto table, int nb, double sc, auto out, auto each, void* l) {
         return diff ? attention_diff_forward_planned(y, p, q, k, v, lam, bucket, table, nb, sc, out, each, l, s.n, s.m, s.H, s.D, c.ws, c.bytes,
                                                      raw(c.stream))
-                    : attention_bucket_forward_planned(y, p, q, k, v, bucket, table, nb, sc, out, l, s.n, s.m, s.H, s.D, c.ws, c.bytes,
+                    : attention_bucket_forward_planned(y, p, q, k, v, bucket, table, nb, sc, out, each, l, s.n, s.m, s.H, s.D, c.ws, c.bytes,
                                                        raw(c.stream));
       });
     });
@@ -787,7 +790,7 @@ TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool d
       return typed(y, [&](auto q, auto k, auto v, auto lam, auto bucket, auto table, int nb, double sc, auto out, auto each, void* l) {
         return diff ? attention_diff_forward(y, i, row, indptr, indices, chunks, q, k, v, lam, bucket, table, nb, sc, out, each, l, e, s.n, s.m,
                                              s.H, s.D, c.ws, c.bytes, raw(c.stream))
-                    : attention_bucket_forward(y, i, row, indptr, indices, chunks, q, k, v, bucket, table, nb, sc, out, l, e, s.n, s.m, s.H, s.D,
+                    : attention_bucket_forward(y, i, row, indptr, indices, chunks, q, k, v, bucket, table, nb, sc, out, each, l, e, s.n, s.m, s.H, s.D,
                                                c.ws, c.bytes, raw(c.stream));
       });
     });
@@ -800,7 +803,7 @@ TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool d
     n.cols = graph.cols;
     n.scale = scale;
     n.save_all({x.q, x.k, x.v, x.lam, x.bucket, x.table, lse});
-    if (diff) n.save(parts);
+    if (parts.defined()) n.save(parts);
     else n.save(o, true);
     if (!graph.planned())
       for (const Tensor& t : graph.t) n.save(t);
@@ -862,15 +865,17 @@ TermsGraph rows_only(const PlanHandle& plan, const Tensor& q) {
   graph.rows = plan.graph;
   return graph;
 }
-std::tuple<Tensor, Tensor> attention_bucket_forward_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Tensor& q,
-                                                     const Tensor& k, const Tensor& v, const Later& bucket, const Later& table, double scale) {
-  const TermsOutputs r = terms_forward(rows_only(row, indptr, indices), {q, k, v, Tensor(), given(bucket), given(table)}, false, scale, false, false);
-  return {r.o, r.lse};
+Values bucket_values(const TermsOutputs& r, bool keep) {
+  return {r.o, r.lse, !keep ? c10::optional<Tensor>() : c10::optional<Tensor>(r.parts.defined() ? r.parts : r.o)};
 }
-std::tuple<Tensor, Tensor> attention_bucket_forward_plan(const PlanHandle& plan, const Tensor& q, const Tensor& k, const Tensor& v,
-                                                         const Later& bucket, const Later& table, double scale) {
-  const TermsOutputs r = terms_forward(rows_only(plan, q), {q, k, v, Tensor(), given(bucket), given(table)}, false, scale, false, false);
-  return {r.o, r.lse};
+Values attention_bucket_forward_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const Tensor& q, const Tensor& k,
+                                 const Tensor& v, const Later& bucket, const Later& table, double scale, bool keep) {
+  return bucket_values(terms_forward(rows_only(row, indptr, indices), {q, k, v, Tensor(), given(bucket), given(table)}, false, scale, false, keep),
+                       keep);
+}
+Values attention_bucket_forward_plan(const PlanHandle& plan, const Tensor& q, const Tensor& k, const Tensor& v, const Later& bucket,
+                                     const Later& table, double scale, bool keep) {
+  return bucket_values(terms_forward(rows_only(plan, q), {q, k, v, Tensor(), given(bucket), given(table)}, false, scale, false, keep), keep);
 }
 Values diff_values(const TermsOutputs& r) {
   return {r.o, r.lse, r.parts.defined() ? c10::optional<Tensor>(r.parts) : c10::nullopt};

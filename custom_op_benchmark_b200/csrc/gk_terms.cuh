@@ -131,7 +131,7 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
   const T* __restrict__ table;   // (buckets, H * kMaps)
   const T* __restrict__ lam;     // (H)
   T* __restrict__ o;
-  T* __restrict__ each;          // (n, H, 2, D): both maps' own sums, for the backward; may be null
+  A* __restrict__ each;          // (n, H, kMaps, D): every map's own sum as it is, for the backward; may be null
   A* __restrict__ lse;           // (n, H * kMaps)
   A scale;
   int buckets;
@@ -228,8 +228,13 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
     for (int i = 0; i < W; ++i) st.q[i].scale(c);
   }
   __device__ __forceinline__ void began(State&, int, bool) const {}
-  __device__ __forceinline__ T* part_row(const State& st, long long node, int m) const {
-    return each + (2 * node * this->HD + (long long)(st.ln.head + m) * this->D + st.ln.off);
+  // o is rounded to the element type, and dO . o out of it would carry that into every score gradient (two-byte elements, 5 edges a
+  // node: dq 2.6e-3 off float64 instead of 1.7e-3): the backward gets the sums unrounded
+  __device__ __forceinline__ void store_sums(const State& st, long long node, int m, const F (&x)[W]) const {
+    A* at = each + (kMaps * node * this->HD + (long long)(kMaps - 1) * st.ln.head * this->D + (long long)m * this->D + st.ln.off);
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (this->has(st.ln, i)) frag_save<A, V>(at + i * this->slot_step(), x[i]);
   }
   __device__ __forceinline__ void store_row(const State& st, int node) const {
     F out[W];
@@ -239,8 +244,7 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
       F x[W];
 #pragma unroll
       for (int i = 0; i < W; ++i) { x[i] = st.acc[m][i]; x[i].scale(inv); }
-      if constexpr (kMaps == 2)
-        if (each) this->store_row_slots(st.ln, part_row(st, node, m), x);
+      if (each) store_sums(st, node, m, x);
       const A c = m == 0 ? A(1) : -to_acc<T>(__ldg(lam + st.ln.head));
 #pragma unroll
       for (int i = 0; i < W; ++i) {
@@ -260,8 +264,7 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
     for (int i = 0; i < W; ++i) z[i].zero();
 #pragma unroll
     for (int m = 0; m < kMaps; ++m) {
-      if constexpr (kMaps == 2)
-        if (each) this->store_row_slots(st.ln, part_row(st, n, m), z);
+      if (each) store_sums(st, n, m, z);
       if (st.ln.first) lse[(n * this->H + st.ln.head) * kMaps + m] = neg_inf<A>();
     }
   }
@@ -308,7 +311,8 @@ struct TermsFwd : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0
 
 // Destination side of the backward: dq, the pairs (p1 - lam p2, g) per position and map, t2 per node for dlam.
 template <class GEO, int kMaps, bool kBucket>
-struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 4 + kTermsMoreDst<GEO, kMaps, kBucket>, 2 + kMaps, kMaps * (int)sizeof(typename GEO::A),
+struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes : 0, 4 + kTermsMoreDst<GEO, kMaps, kBucket>,
+                            2 + kMaps * (int)(sizeof(typename GEO::A) / sizeof(typename GEO::T)), kMaps * (int)sizeof(typename GEO::A),
                             (sizeof(typename GEO::T) == 2 ? 2 : 1), true> {
   using T = typename GEO::T;
   using A = typename GEO::A;
@@ -316,7 +320,8 @@ struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes 
   using Scores = TermsScores<GEO, kMaps>;
   using Bias = TermsBias<GEO, kMaps>;
   using Raw = typename Bias::Raw;
-  static constexpr int W = GEO::W, V = GEO::V, kRow = GEO::kRow;   // rows of a ring step: k, v; of a node: q, dO, o of every map
+  static constexpr int W = GEO::W, V = GEO::V, kRow = GEO::kRow;   // rows of a ring step: k, v; of a node: q, dO, the sum of every map
+  static constexpr int kPer = (int)(sizeof(A) / sizeof(T));        // rows that a sum's row of wider elements fills
   static constexpr const char* kName = kMaps == 2 ? "attention_diff_bwd_dst" : "attention_bucket_bwd_dst";
   static constexpr bool kRowOut = true, kUsesOther = true, kUsesEid = kBucket, kFoldsEid = false, kComputed = kBucket, kMasks = kBucket;
   const T* __restrict__ q;
@@ -324,7 +329,7 @@ struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes 
   const T* __restrict__ v;
   const T* __restrict__ table;
   const T* __restrict__ lam;
-  const T* __restrict__ o;         // (n, H, kMaps, D)
+  const A* __restrict__ sums;      // (n, H, kMaps, D), unrounded
   const T* __restrict__ dout;
   const A* __restrict__ lse;
   EdgePair<A>* __restrict__ pd;    // (E, Hp)
@@ -410,10 +415,16 @@ struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes 
     this->stage_row(st.ln, buf, reinterpret_cast<const unsigned char*>(q + st.ln.off), node, this->rowb, true);
     this->stage_row(st.ln, buf + kRow, reinterpret_cast<const unsigned char*>(dout + st.ln.off), node, this->rowb, true);
 #pragma unroll
-    for (int m = 0; m < kMaps; ++m) {
-      const T* at = kMaps == 1 ? o + st.ln.off : o + ((long long)(st.ln.head + m) * this->D + st.ln.off);
-      this->stage_row(st.ln, buf + (2 + m) * kRow, reinterpret_cast<const unsigned char*>(at), node, kMaps * this->rowb, true);
-    }
+    for (int m = 0; m < kMaps; ++m)
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const A* at = sums + ((long long)(kMaps - 1) * st.ln.head * this->D + (long long)m * this->D + st.ln.off) + j * (V / kPer);
+        const unsigned char* from = reinterpret_cast<const unsigned char*>(at) + (unsigned long long)(unsigned)node * (kMaps * kPer * this->rowb);
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          cp_async_slot<GEO::SB>(buf + (2 + m * kPer + j) * kRow + i * 32 * GEO::SB, from + (size_t)(i * this->slot_step()) * sizeof(A),
+                                 this->has(st.ln, i));
+      }
     cp_async_slot<kMaps * sizeof(A)>(buf + lse_at(lane), lse + ((long long)node * this->H + st.ln.head) * kMaps, true);
   }
   __device__ __forceinline__ void begin(State& st, unsigned buf, int lane) const {
@@ -424,7 +435,19 @@ struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes 
 #pragma unroll
     for (int m = 0; m < kMaps; ++m) {
       lds(st.lse2[m], buf + lse_at(lane) + m * (int)sizeof(A));
-      this->load_staged(ov, buf + (2 + m) * kRow);
+      if constexpr (kPer == 1) {
+        this->load_staged(ov, buf + (2 + m) * kRow);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            Frag<A, V / kPer> half;
+            frag_lds<A, GEO::SB>(half, buf + (2 + m * kPer + j) * kRow + i * 32 * GEO::SB);
+#pragma unroll
+            for (int k = 0; k < V / kPer / 2; ++k) ov[i].p[j * (V / kPer / 2) + k] = half.p[k];
+          }
+      }
       st.delta[m] = frag_dot<V, W>(st.gr, ov);   // this lane's part: summed in began()
     }
     const A c = scale * A(kLog2e);
@@ -684,11 +707,11 @@ struct TermsCall {
 // Defined in gk_terms_banded.cuh for bfloat16: the tensor-core kernels for dense-band graphs; GRAPHOP_ERR_UNSUPPORTED when the call is
 // not one they take.
 template <typename T>
-inline int banded_terms_forward(const graphop_plan_t*, const TermsCall<T>&, T*, T*, void*, void*, size_t, cudaStream_t) {
+inline int banded_terms_forward(const graphop_plan_t*, const TermsCall<T>&, T*, void*, void*, void*, size_t, cudaStream_t) {
   return GRAPHOP_ERR_UNSUPPORTED;
 }
 template <typename T>
-inline int banded_terms_backward(const graphop_plan_t*, const graphop_plan_t*, const TermsCall<T>&, const T*, const void*, const T*, T*,
+inline int banded_terms_backward(const graphop_plan_t*, const graphop_plan_t*, const TermsCall<T>&, const void*, const void*, const T*, T*,
                                  T*, T*, T*, T*, void*, size_t, cudaStream_t) {
   return GRAPHOP_ERR_UNSUPPORTED;
 }
@@ -719,30 +742,30 @@ inline int terms_check(const TermsCall<T>& c, long long C, bool al, GeoPick* geo
 inline bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 template <typename T, int kMaps, bool kBucket>
-inline int run_terms_forward(Arena& ar, const GraphView& g, const GeoPick& s, const TermsCall<T>& c, T* o, T* parts, void* lse,
+inline int run_terms_forward(Arena& ar, const GraphView& g, const GeoPick& s, const TermsCall<T>& c, T* o, void* sums, void* lse,
                              cudaStream_t st) {
   return dispatch_geo<T, false, true>(s, [&](auto tag) -> int {
     TermsFwd<typename decltype(tag)::type, kMaps, kBucket> op;
     using A = typename decltype(op)::A;
     fill_geo(op, s, c.H, c.row_d());
-    op.q = c.q; op.k = c.k; op.v = c.v; op.table = c.table; op.lam = c.lam; op.o = o; op.each = parts; op.lse = (A*)lse;
+    op.q = c.q; op.k = c.k; op.v = c.v; op.table = c.table; op.lam = c.lam; op.o = o; op.each = (A*)sums; op.lse = (A*)lse;
     op.scale = (A)c.scale; op.buckets = c.buckets;
     return launch_walk(ar, g, s, op, c.n_dst, tiles_near(2 * (long long)c.node_bytes(c.n_src)), st);
   });
 }
 
 template <typename T, class GS>
-inline int terms_forward(const GS& gs, long long C, const TermsCall<T>& c, T* o, T* parts, void* lse, void* ws, size_t wsb,
+inline int terms_forward(const GS& gs, long long C, const TermsCall<T>& c, T* o, void* sums, void* lse, void* ws, size_t wsb,
                          cudaStream_t st) {
   using A = typename AccOf<T>::type;
   GeoPick s;
-  const bool al = aligned16(c.q) && aligned16(c.k) && aligned16(c.v) && aligned16(o) && aligned16(parts);
+  const bool al = aligned16(c.q) && aligned16(c.k) && aligned16(c.v) && aligned16(o) && aligned16(sums);
   GK_TRY(terms_check(c, C, al, &s));
   if (c.n_dst == 0) return c.E ? GRAPHOP_ERR_INVALID_ARGUMENT : GRAPHOP_OK;
   if (!o || !lse || !aligned_to(lse, c.maps() * sizeof(A))) return GRAPHOP_ERR_INVALID_ARGUMENT;
   if (c.E == 0) {   // no edge anywhere
     GK_CUDA(cudaMemsetAsync(o, 0, c.node_bytes(c.n_dst), st));
-    if (parts) GK_CUDA(cudaMemsetAsync(parts, 0, 2 * c.node_bytes(c.n_dst), st));
+    if (sums) GK_CUDA(cudaMemsetAsync(sums, 0, c.maps() * c.node_bytes(c.n_dst) / sizeof(T) * sizeof(A), st));
     const long long cells = c.n_dst * c.H * c.maps();
     fill_kernel<A><<<(unsigned)((cells + 255) / 256 < 4096 ? (cells + 255) / 256 : 4096), 256, 0, st>>>((A*)lse, neg_inf_host<A>(), cells);
     GK_LAUNCHED("fill");
@@ -752,25 +775,25 @@ inline int terms_forward(const GS& gs, long long C, const TermsCall<T>& c, T* o,
     return GRAPHOP_ERR_INVALID_ARGUMENT;
   GK_TRY(check_ws(ws));
   if constexpr (std::is_same_v<GS, FromPlan>) {
-    const int rc = banded_terms_forward<T>(gs.p, c, o, parts, lse, ws, wsb, st);
+    const int rc = banded_terms_forward<T>(gs.p, c, o, sums, lse, ws, wsb, st);
     if (rc != GRAPHOP_ERR_UNSUPPORTED) return rc;
   }
   Arena ar(ws, wsb);
   GraphView g;
   GK_TRY(gs(ar, c.n_dst, st, &g));
   g.eid = c.buckets ? c.bucket : nullptr;
-  if (!c.diff) return run_terms_forward<T, 1, true>(ar, g, s, c, o, nullptr, lse, st);
-  if (c.buckets) return run_terms_forward<T, 2, true>(ar, g, s, c, o, parts, lse, st);
-  return run_terms_forward<T, 2, false>(ar, g, s, c, o, parts, lse, st);
+  if (!c.diff) return run_terms_forward<T, 1, true>(ar, g, s, c, o, sums, lse, st);
+  if (c.buckets) return run_terms_forward<T, 2, true>(ar, g, s, c, o, sums, lse, st);
+  return run_terms_forward<T, 2, false>(ar, g, s, c, o, sums, lse, st);
 }
 
 template <typename T, int kMaps, bool kBucket, class A>
-inline int run_terms_dst(Arena& ar, const GraphView& g, const GeoPick& s, const TermsCall<T>& c, const T* o, const void* lse,
+inline int run_terms_dst(Arena& ar, const GraphView& g, const GeoPick& s, const TermsCall<T>& c, const void* sums, const void* lse,
                          const T* dout, EdgePair<A>* pd, int Hp, A* t2, T* dq, cudaStream_t st) {
   return dispatch_geo<T, false, true>(s, [&](auto tag) -> int {
     TermsBwdDst<typename decltype(tag)::type, kMaps, kBucket> op;
     fill_geo(op, s, c.H, c.row_d());
-    op.q = c.q; op.k = c.k; op.v = c.v; op.table = c.table; op.lam = c.lam; op.o = o; op.dout = dout; op.lse = (const A*)lse;
+    op.q = c.q; op.k = c.k; op.v = c.v; op.table = c.table; op.lam = c.lam; op.sums = (const A*)sums; op.dout = dout; op.lse = (const A*)lse;
     op.pd = pd; op.t2 = t2; op.dq = dq; op.scale = (A)c.scale; op.Hp = Hp; op.buckets = c.buckets;
     return launch_walk(ar, g, s, op, c.n_dst, tiles_near(2 * (long long)c.node_bytes(c.n_src)), st);
   });
@@ -808,15 +831,15 @@ inline int run_terms_src(Arena& ar, const GraphView& g, const TermsCall<T>& c, c
   }
 }
 
-// o: the forward's output (bucket), or its parts (diff).  The transposed CSR carries edge ids: for each of its positions the row-CSR
+// sums: what the forward left in `sums`, or its output where that is the accumulator type.  The transposed CSR carries edge ids: for each of its positions the row-CSR
 // position of the same edge.
 template <typename T, class GS>
-inline int terms_backward(const GS& gs_r, const GS& gs_c, bool has_eid_t, long long C, long long Ct, const TermsCall<T>& c, const T* o,
+inline int terms_backward(const GS& gs_r, const GS& gs_c, bool has_eid_t, long long C, long long Ct, const TermsCall<T>& c, const void* sums,
                           const void* lse, const T* dout, T* dq, T* dk, T* dv, T* d_table, T* d_lam, void* ws, size_t wsb,
                           cudaStream_t st) {
   using A = typename AccOf<T>::type;
   GeoPick s;
-  const bool al = aligned16(c.q) && aligned16(c.k) && aligned16(c.v) && aligned16(o) && aligned16(dout) && aligned16(dq) &&
+  const bool al = aligned16(c.q) && aligned16(c.k) && aligned16(c.v) && aligned16(sums) && aligned16(dout) && aligned16(dq) &&
                   aligned16(dk) && aligned16(dv);
   GK_TRY(terms_check(c, C, al, &s));
   if (Ct < 0 || (c.n_dst && !dq) || (c.n_src && (!dk || !dv)) || (c.buckets && !d_table) || (c.diff && !d_lam))
@@ -830,12 +853,12 @@ inline int terms_backward(const GS& gs_r, const GS& gs_c, bool has_eid_t, long l
     if (c.diff) GK_CUDA(cudaMemsetAsync(d_lam, 0, (size_t)c.H * sizeof(T), st));
     return GRAPHOP_OK;
   }
-  if (!has_eid_t || !gs_r.valid(true) || !gs_c.valid(true) || !c.q || !c.k || !c.v || !o || !lse || !dout || !c.n_dst || !c.n_src ||
+  if (!has_eid_t || !gs_r.valid(true) || !gs_c.valid(true) || !c.q || !c.k || !c.v || !sums || !lse || !dout || !c.n_dst || !c.n_src ||
       (c.diff && !c.lam) || (c.buckets && (!c.bucket || !c.table)) || !aligned_to(lse, c.maps() * sizeof(A)))
     return GRAPHOP_ERR_INVALID_ARGUMENT;
   GK_TRY(check_ws(ws));
   if constexpr (std::is_same_v<GS, FromPlan>) {
-    const int rc = banded_terms_backward<T>(gs_r.p, gs_c.p, c, o, lse, dout, dq, dk, dv, d_table, d_lam, ws, wsb, st);
+    const int rc = banded_terms_backward<T>(gs_r.p, gs_c.p, c, sums, lse, dout, dq, dk, dv, d_table, d_lam, ws, wsb, st);
     if (rc != GRAPHOP_ERR_UNSUPPORTED) return rc;
   }
   Arena ar(ws, wsb);
@@ -847,9 +870,9 @@ inline int terms_backward(const GS& gs_r, const GS& gs_c, bool has_eid_t, long l
     GraphView g;
     GK_TRY(gs_r(ar, c.n_dst, st, &g));
     g.eid = c.buckets ? c.bucket : nullptr;
-    if (!c.diff) GK_TRY((run_terms_dst<T, 1, true>(ar, g, s, c, o, lse, dout, pd, Hp, t2, dq, st)));
-    else if (c.buckets) GK_TRY((run_terms_dst<T, 2, true>(ar, g, s, c, o, lse, dout, pd, Hp, t2, dq, st)));
-    else GK_TRY((run_terms_dst<T, 2, false>(ar, g, s, c, o, lse, dout, pd, Hp, t2, dq, st)));
+    if (!c.diff) GK_TRY((run_terms_dst<T, 1, true>(ar, g, s, c, sums, lse, dout, pd, Hp, t2, dq, st)));
+    else if (c.buckets) GK_TRY((run_terms_dst<T, 2, true>(ar, g, s, c, sums, lse, dout, pd, Hp, t2, dq, st)));
+    else GK_TRY((run_terms_dst<T, 2, false>(ar, g, s, c, sums, lse, dout, pd, Hp, t2, dq, st)));
     if (c.buckets)
       GK_TRY((run_bucket_sum<T>(ar, &pd->ds, c.E, 2ll * Hp, 2, columns, c.bucket, c.buckets, g.hdr, 1.0, d_table, st)));
     if (c.diff) GK_TRY((run_bucket_sum<T>(ar, t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));

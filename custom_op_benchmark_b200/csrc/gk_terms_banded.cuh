@@ -10,8 +10,9 @@
 // order the threads of a tile read them, 255 where an element takes no part or lies outside the band; the head's column of the
 // table waits in shared memory with -inf at 255, so that the masks and the band's edge need no tests.
 //
-// dT sums the score gradients by bucket: the destination side stores them as bfloat16 (they are rounded to it for the product
-// with k as well) in the tiles' order, and band_bucket_sum_kernel adds them up, a private table per thread.
+// dT sums the score gradients by bucket: the destination side stores them with 16 bits of mantissa, in two planes (as bfloat16, to
+// which they are rounded for the product with k, a sum of gradients of either sign was 2.4e-3 off float64, of which the stored dT's own
+// rounding is 1.7e-3) in the tiles' order, and band_bucket_sum_kernel adds them up, a private table per thread.
 //
 // A product takes whole blocks: 0 * NaN from a row that takes no part, or that lies next to the band, reaches every row of the
 // tile.  A tile that ends with a value that is not finite says so in `dirty`, and band_again_kernel does it again edge by edge.
@@ -36,11 +37,12 @@ struct TermsTile {
   int H;
   float scale;
   // forward
-  __nv_bfloat16 *o, *parts;
-  float* lse;
+  __nv_bfloat16* o;
+  float *sums, *lse;                         // (n, H, maps, 64) unrounded, may be null; (n, H, maps)
   // backward
   float2* stat;                              // (n_dst, H, maps): (lse in base-2 units, dO . o)
-  __nv_bfloat16* g;                          // (H, maps, tiles, pitch / 32, 128, 32): score gradients
+  unsigned short* g;                         // (H, maps, tiles, pitch / 32, 128, 32): upper halves of the score gradients
+  unsigned char* g_low;                      // and the next 8 bits
   __nv_bfloat16 *out0, *out1;                // dq | dk, dv
 };
 
@@ -410,7 +412,11 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           o[j] = !ok ? NAN : l[m] == 0.f ? 0.f : o[j] * inv[m];
           out[j] = m == 0 ? o[j] : fmaf(-lam, o[j], out[j]);
         }
-        if (kMaps == 2 && p.parts && r < p.n_own) store16(p.parts + (((long long)r * p.H + head) * 2 + m) * kD + f0, o);
+        if (p.sums && r < p.n_own) {
+          float4* at = reinterpret_cast<float4*>(p.sums + (((long long)r * p.H + head) * kMaps + m) * kD + f0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) at[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
       }
       if (r < p.n_own) store16(p.o + ((long long)r * p.H + head) * kD + f0, out);
     }
@@ -427,11 +433,9 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 #pragma unroll
     for (int q = 0; q < kD / 8; ++q) {
       *reinterpret_cast<uint4*>(p.o + ((long long)r * p.H + head) * kD + q * 8) = zero;
-      if (kMaps == 2 && p.parts) {
-        *reinterpret_cast<uint4*>(p.parts + ((long long)r * p.H + head) * 2 * kD + q * 8) = zero;
-        *reinterpret_cast<uint4*>(p.parts + (((long long)r * p.H + head) * 2 + 1) * kD + q * 8) = zero;
-      }
     }
+    if (p.sums)
+      for (int q = 0; q < kMaps * kD / 4; ++q) *reinterpret_cast<uint4*>(p.sums + ((long long)r * p.H + head) * kMaps * kD + q * 4) = zero;
 #pragma unroll
     for (int m = 0; m < kMaps; ++m) p.lse[((long long)r * p.H + head) * kMaps + m] = -INFINITY;
   }
@@ -600,6 +604,7 @@ __device__ __forceinline__ void terms_backward_tile(const CUtensorMap& map_a, co
 #pragma unroll
       for (int half = 0; half < kC / 16; ++half) {
         uint32_t pw[8], pg[kMaps][8];
+        [[maybe_unused]] uint32_t up[kMaps][8], low[kMaps][4];
         if (live) {
           uint32_t raw[kMaps + 1][16];
 #pragma unroll
@@ -627,14 +632,25 @@ __device__ __forceinline__ void terms_backward_tile(const CUtensorMap& map_a, co
             if constexpr (kSrc) pw[j / 2] = pack_bf16(w[0], w[1]);
 #pragma unroll
             for (int m = 0; m < kMaps; ++m) pg[m][j / 2] = pack_bf16(g[m][0], g[m][1]);
+            if constexpr (kBucket && !kSrc) {   // bits 31-16 and 15-8 of both, the latter four elements to a word
+#pragma unroll
+              for (int m = 0; m < kMaps; ++m) {
+                const uint32_t x = __float_as_uint(g[m][0]), y = __float_as_uint(g[m][1]);
+                up[m][j / 2] = __byte_perm(x, y, 0x7632);
+                const uint32_t two = __byte_perm(x, y, 0x0051);
+                if (j & 2) low[m][j / 4] |= two << 16;
+                else low[m][j / 4] = two & 0xffffu;
+              }
+            }
           }
           if constexpr (kBucket && !kSrc) {
 #pragma unroll
             for (int m = 0; m < kMaps; ++m) {
-              uint4* at = reinterpret_cast<uint4*>(p.g + ((size_t)(head * kMaps + m) * tiles * p.pitch * kTileM + tile_at +
-                                                         (size_t)(2 * b + cg) * kC * kTileM + row * kC + half * 16));
-              at[0] = make_uint4(pg[m][0], pg[m][1], pg[m][2], pg[m][3]);
-              at[1] = make_uint4(pg[m][4], pg[m][5], pg[m][6], pg[m][7]);
+              const size_t to = (size_t)(head * kMaps + m) * tiles * p.pitch * kTileM + tile_at + (size_t)(2 * b + cg) * kC * kTileM + row * kC + half * 16;
+              uint4* at = reinterpret_cast<uint4*>(p.g + to);
+              at[0] = make_uint4(up[m][0], up[m][1], up[m][2], up[m][3]);
+              at[1] = make_uint4(up[m][4], up[m][5], up[m][6], up[m][7]);
+              *reinterpret_cast<uint4*>(p.g_low + to) = make_uint4(low[m][0], low[m][1], low[m][2], low[m][3]);
             }
           }
         } else {
@@ -736,7 +752,7 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // A row of which nothing took part has no probabilities, whatever dO holds.
 template <int kMaps>
 __global__ void __launch_bounds__(256)
-band_stat_kernel(const __nv_bfloat16* __restrict__ sums, const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse, long long cells,
+band_stat_kernel(const float* __restrict__ sums, const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse, long long cells,
                  float2* __restrict__ stat, float* __restrict__ t2) {
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
   const int part = threadIdx.x & 7;
@@ -749,12 +765,13 @@ band_stat_kernel(const __nv_bfloat16* __restrict__ sums, const __nv_bfloat16* __
     const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv);
 #pragma unroll
     for (int m = 0; m < kMaps; ++m) {
-      const uint4 ov = __ldg(reinterpret_cast<const uint4*>(sums + (i * kMaps + m) * kD) + part);
-      const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&ov);
+      const float4* at = reinterpret_cast<const float4*>(sums + (i * kMaps + m) * kD) + 2 * part;
+      const float4 x = __ldg(at), y = __ldg(at + 1);
+      const float of[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 of = __bfloat1622float2(o2[e]), gf = __bfloat1622float2(g2[e]);
-        d[m] += of.x * gf.x + of.y * gf.y;
+        const float2 gf = __bfloat1622float2(g2[e]);
+        d[m] += of[2 * e] * gf.x + of[2 * e + 1] * gf.y;
       }
     }
   }
@@ -863,7 +880,7 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
 #pragma unroll
         for (int m = 0; m < kMaps; ++m) {
           const float inv = l[m] == 0.f ? 0.f : 1.f / l[m], e0 = acc[m][0] * inv, e1 = acc[m][1] * inv, cm = m == 0 ? 1.f : -lam;
-          if (kMaps == 2 && t.parts) put(t.parts, 2 * at + m, e0, e1);
+          if (t.sums) *reinterpret_cast<float2*>(t.sums + (at * kMaps + m) * kD + 2 * lane) = make_float2(e0, e1);
           o0 = fmaf(cm, e0, o0);
           o1 = fmaf(cm, e1, o1);
           if (lane == 0) t.lse[at * kMaps + m] = (mx[m] + log2f(l[m])) * (float)kLn2;
@@ -886,25 +903,30 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
 // per element and the table's stride not known, 14: 36 us for 6.3M elements of 8 heads), then by reading the gradients.
 template <int NT>
 __global__ void __launch_bounds__(NT)
-band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const __nv_bfloat16* __restrict__ g, long long elements, int buckets,
-                       int columns, double* __restrict__ partial) {
+band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const unsigned short* __restrict__ g, const unsigned char* __restrict__ g_low,
+                       long long elements, int buckets, int columns, double* __restrict__ partial) {
   extern __shared__ float cells[];
   constexpr int kAhead = 4;
   const int tid = threadIdx.x, column = blockIdx.y;
   const long long pieces = elements / 8, stride = (long long)gridDim.x * NT;
   const uint2* idp = reinterpret_cast<const uint2*>(ids);
   const uint4* src = reinterpret_cast<const uint4*>(g + (size_t)column * elements);
+  const uint2* src_low = reinterpret_cast<const uint2*>(g_low + (size_t)column * elements);
   float* mine = cells + tid;
   for (int b = 0; b <= buckets; ++b) mine[b * NT] = 0.f;
   const unsigned none = (unsigned)buckets;
   for (long long i = (long long)blockIdx.x * NT + tid; i < pieces; i += kAhead * stride) {
     uint2 id[kAhead];
     uint4 w[kAhead];
+    uint2 l[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) id[k] = i + k * stride < pieces ? __ldg(idp + i + k * stride) : make_uint2(0xffffffffu, 0xffffffffu);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if ((id[k].x & id[k].y) != 0xffffffffu) w[k] = __ldg(src + i + k * stride);   // else nothing takes part, and nothing was stored
+      if ((id[k].x & id[k].y) != 0xffffffffu) {   // else nothing takes part, and nothing was stored
+        w[k] = __ldg(src + i + k * stride);
+        l[k] = __ldg(src_low + i + k * stride);
+      }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if ((id[k].x & id[k].y) == 0xffffffffu) continue;
@@ -912,7 +934,9 @@ band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const __nv_bfloat1
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const unsigned b = min(((j < 4 ? id[k].x : id[k].y) >> (8 * (j & 3))) & 255u, none);
-        mine[b * NT] += __uint_as_float((j & 1) ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
+        // bytes of the float, from the highest: two of the upper plane, one of the lower, zero
+        const unsigned high = (j & 1) ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16, next = j < 4 ? l[k].x : l[k].y;
+        mine[b * NT] += __uint_as_float(__byte_perm(high, next, 0x3200 | ((4 + (j & 3)) << 4)));
       }
     }
   }
@@ -941,11 +965,11 @@ inline BandSumShape band_sum_shape(long long elements, int buckets, int columns)
   s.blocks = (int)blocks;
   return s;
 }
-inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, const __nv_bfloat16* g, long long elements, int buckets,
-                               int columns, double* partial, __nv_bfloat16* out, cudaStream_t st) {
+inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, const unsigned short* g, const unsigned char* g_low,
+                               long long elements, int buckets, int columns, double* partial, __nv_bfloat16* out, cudaStream_t st) {
   const auto launch = [&](auto kernel, std::atomic<bool> (&configured)[64]) -> int {
     GK_TRY(allow_smem(kernel, 56 * 1024, configured));
-    kernel<<<dim3((unsigned)s.blocks, (unsigned)columns), s.threads, s.smem, st>>>(ids, g, elements, buckets, columns, partial);
+    kernel<<<dim3((unsigned)s.blocks, (unsigned)columns), s.threads, s.smem, st>>>(ids, g, g_low, elements, buckets, columns, partial);
     GK_LAUNCHED("band_bucket_sum");
     return GRAPHOP_OK;
   };
@@ -997,7 +1021,7 @@ inline int run_band_again(const AgainArgs& a, cudaStream_t st) {
 }
 
 template <int kMaps, bool kBucket>
-inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat16>& c, __nv_bfloat16* o, __nv_bfloat16* parts, void* lse,
+inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat16>& c, __nv_bfloat16* o, void* sums, void* lse,
                          Arena& ar, cudaStream_t st) {
   using L = FwdLayout<kMaps>;
   const int pitch = band_pitch(plan);
@@ -1013,7 +1037,7 @@ inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat
   GK_TRY(allow_smem(terms_forward_kernel<kMaps, kBucket>, L::kBytes, configured));
   if (kBucket) GK_TRY(run_band_ids(band_ids_of(plan, nullptr, c.n_dst, 32, const_cast<unsigned char*>(t.ids)), nullptr, c.bucket, c.buckets, st));
   t.table = c.table; t.lam = c.lam; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan->node_lo; t.node_deg = plan->node_deg;
-  t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.o = o; t.parts = parts; t.lse = (float*)lse;
+  t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.o = o; t.sums = (float*)sums; t.lse = (float*)lse;
   terms_forward_kernel<kMaps, kBucket><<<dim3((unsigned)tiles, (unsigned)c.H), kThreads, L::kBytes, st>>>(mq, mk, mv, t);
   GK_LAUNCHED(kMaps == 2 ? "attention_diff_fwd_banded" : "attention_bucket_fwd_banded");
   const AgainArgs a{t, c.q, c.k, c.v, nullptr, plan->node_first, nullptr, c.bucket, (int)tiles};
@@ -1022,7 +1046,7 @@ inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat
 
 template <int kMaps, bool kBucket>
 inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* plan_t, const TermsCall<__nv_bfloat16>& c,
-                          const __nv_bfloat16* sums, const void* lse, const __nv_bfloat16* dout, __nv_bfloat16* dq, __nv_bfloat16* dk,
+                          const void* sums, const void* lse, const __nv_bfloat16* dout, __nv_bfloat16* dq, __nv_bfloat16* dk,
                           __nv_bfloat16* dv, __nv_bfloat16* d_table, __nv_bfloat16* d_lam, Arena& ar, cudaStream_t st) {
   using LD = BwdLayout<false, kMaps>;
   using LS = BwdLayout<true, kMaps>;
@@ -1040,7 +1064,8 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   if (kBucket) {
     ids = (unsigned char*)ar.take((size_t)elements);
     ids_t = (unsigned char*)ar.take((size_t)tiles_t * pitch_t * kTileM);
-    t.g = (__nv_bfloat16*)ar.take((size_t)columns * elements * sizeof(__nv_bfloat16));
+    t.g = (unsigned short*)ar.take((size_t)columns * elements * 2);
+    t.g_low = (unsigned char*)ar.take((size_t)columns * elements);
     partial = (double*)ar.take((size_t)sum.blocks * c.buckets * columns * sizeof(double));
   }
   const size_t before_sum = ar.used;
@@ -1060,7 +1085,7 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
     GK_TRY(run_band_ids(band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, ids), &other, c.bucket, c.buckets, st));
   }
   const long long cells = c.n_dst * c.H;
-  band_stat_kernel<kMaps><<<(unsigned)((cells * 8 + 255) / 256), 256, 0, st>>>(sums, dout, (const float*)lse, cells, t.stat, t2);
+  band_stat_kernel<kMaps><<<(unsigned)((cells * 8 + 255) / 256), 256, 0, st>>>((const float*)sums, dout, (const float*)lse, cells, t.stat, t2);
   GK_LAUNCHED("band_stat");
   t.table = c.table; t.lam = c.lam; t.ids = ids; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan_r->node_lo;
   t.node_deg = plan_r->node_deg; t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.out0 = dq;
@@ -1072,7 +1097,7 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   GK_LAUNCHED(kMaps == 2 ? "attention_diff_bwd_banded" : "attention_bucket_bwd_banded");
   GK_TRY((run_band_again<1, kMaps, kBucket>(AgainArgs{t, c.q, c.k, c.v, dout, plan_r->node_first, nullptr, c.bucket, (int)tiles}, st)));
   GK_TRY((run_band_again<2, kMaps, kBucket>(AgainArgs{u, c.q, c.k, c.v, dout, plan_t->node_first, plan_t->eid, c.bucket, (int)tiles_t}, st)));
-  if (kBucket) GK_TRY(run_band_bucket_sum(sum, ids, t.g, elements, c.buckets, columns, partial, d_table, st));
+  if (kBucket) GK_TRY(run_band_bucket_sum(sum, ids, t.g, t.g_low, elements, c.buckets, columns, partial, d_table, st));
   if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));
   return GRAPHOP_OK;
 }
@@ -1084,17 +1109,17 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
 // GRAPHOP_ERR_UNSUPPORTED else: the caller then runs the walkers.
 template <>
 inline int banded_terms_forward<__nv_bfloat16>(const graphop_plan_t* plan, const TermsCall<__nv_bfloat16>& c, __nv_bfloat16* o,
-                                               __nv_bfloat16* parts, void* lse, void* ws, size_t wsb, cudaStream_t st) {
+                                               void* sums, void* lse, void* ws, size_t wsb, cudaStream_t st) {
   if (c.row_d() != banded::kD || c.buckets > banded::kMostBandBuckets || c.n_src < 1 || !banded::band_plan_ok(plan, c.n_dst, c.H))
     return GRAPHOP_ERR_UNSUPPORTED;
   Arena ar(ws, wsb);
-  if (!c.diff) return banded::terms_forward<1, true>(plan, c, o, nullptr, lse, ar, st);
-  if (c.buckets) return banded::terms_forward<2, true>(plan, c, o, parts, lse, ar, st);
-  return banded::terms_forward<2, false>(plan, c, o, parts, lse, ar, st);
+  if (!c.diff) return banded::terms_forward<1, true>(plan, c, o, sums, lse, ar, st);
+  if (c.buckets) return banded::terms_forward<2, true>(plan, c, o, sums, lse, ar, st);
+  return banded::terms_forward<2, false>(plan, c, o, sums, lse, ar, st);
 }
 template <>
 inline int banded_terms_backward<__nv_bfloat16>(const graphop_plan_t* plan_r, const graphop_plan_t* plan_t,
-                                                const TermsCall<__nv_bfloat16>& c, const __nv_bfloat16* sums, const void* lse,
+                                                const TermsCall<__nv_bfloat16>& c, const void* sums, const void* lse,
                                                 const __nv_bfloat16* dout, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv,
                                                 __nv_bfloat16* d_table, __nv_bfloat16* d_lam, void* ws, size_t wsb, cudaStream_t st) {
   if (c.row_d() != banded::kD || c.buckets > banded::kMostBandBuckets || !banded::band_plan_ok(plan_r, c.n_dst, c.H) ||

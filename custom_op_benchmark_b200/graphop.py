@@ -888,7 +888,7 @@ def _plan_both(plan_r, plan_t, n_dst, n_src):
     return (None, 4, [plan_r.ref(), plan_t.ref()]), plan_r.n_edges
 
 
-def _bucket_forward(graph, e, q, k, v, bucket, table, scale):
+def _bucket_forward(graph, e, q, k, v, bucket, table, scale, keep_sums):
     if bucket is None or table is None:
         raise RuntimeError("bucket and table must be given")
     _check_all(q=q, k=k, v=v)
@@ -897,31 +897,34 @@ def _bucket_forward(graph, e, q, k, v, bucket, table, scale):
     h, d = _terms_shape(q, k, v, False)
     nb = _terms_bias(bucket, table, h, e, q.device)
     o = th.empty_like(q)
+    sums = th.empty_like(q, dtype=_lse_dtype(q)) if keep_sums and q.dtype != _lse_dtype(q) else None
     lse = th.empty((q.size(0), h), dtype=_lse_dtype(q), device=q.device)
     _terms_call("attention_bucket_forward", graph, elem, _capi.TERMS_BUCKET_FWD, e, max(q.size(0), k.size(0)), h, d, nb, q.device,
-                [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, float(scale), _p(o), _p(lse)] + ([] if graph[0] is None else [e])
+                [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, float(scale), _p(o), _p(sums), _p(lse)] + ([] if graph[0] is None else [e])
                 + [q.size(0), k.size(0), h, d])
-    return o, lse
+    return (o, lse, o if sums is None else sums) if keep_sums else (o, lse)
 
 
-def _bucket_backward(graph, e, q, k, v, bucket, table, o, lse, d_o, scale):
+def _bucket_backward(graph, e, q, k, v, bucket, table, sums, lse, d_o, scale):
     d_o = d_o.contiguous()
-    _check_all(q=q, k=k, v=v, o=o, lse=lse, d_o=d_o)
-    elem = _elem(q, k, v, table, o, d_o)
-    _same_device(q, k, v, o, lse, d_o)
+    _check_all(q=q, k=k, v=v, sums=sums, lse=lse, d_o=d_o)
+    elem = _elem(q, k, v, table, d_o)
+    _same_device(q, k, v, sums, lse, d_o)
     h, d = _terms_shape(q, k, v, False)
     nb = _terms_bias(bucket, table, h, e, q.device)
-    if o.shape != q.shape or d_o.shape != q.shape or lse.numel() != q.size(0) * h or lse.dtype != _lse_dtype(q):
-        raise RuntimeError("o, lse and d_o must have the forward's shapes and types")
+    if sums.shape != q.shape or sums.dtype != _lse_dtype(q) or d_o.shape != q.shape or lse.numel() != q.size(0) * h \
+            or lse.dtype != _lse_dtype(q):
+        raise RuntimeError("sums, lse and d_o must have the forward's shapes and types")
     out = [th.empty_like(t) for t in (q, k, v, table)]
     _terms_call("attention_bucket_backward", graph, elem, _capi.TERMS_BUCKET_BWD, e, max(q.size(0), k.size(0)), h, d, nb, q.device,
-                [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, _p(o), _p(lse), _p(d_o), float(scale)] + [_p(t) for t in out]
+                [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, _p(sums), _p(lse), _p(d_o), float(scale)] + [_p(t) for t in out]
                 + ([] if graph[0] is None else [e]) + [q.size(0), k.size(0), h, d])
     return out
 
 
-def attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale):
-    """(o, lse): attention_forward with a learned bias by buckets in the scores, scale * q[n].k[indices[j]] +
+def attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale, keep_sums=False):
+    """(o, lse), and with ``keep_sums`` what the backward reads, the output before it is rounded (float32 for bfloat16, else o
+    itself): attention_forward with a learned bias by buckets in the scores, scale * q[n].k[indices[j]] +
     table[bucket[j], h] for position j of the row CSR.  ``bucket`` (e,) int32 (``relative_buckets`` makes them of positions; an
     edge type or a hop distance serves as well), ``table`` (buckets, h) of the node tensors' type.
 
@@ -930,31 +933,33 @@ def attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale
     lse = -inf.  One destination per sequence and its cached rows as sources, in any order, make a decoding step."""
     native = native_functions_if_built()
     if native is not None:
-        return native.attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale)
+        out = native.attention_bucket_forward(row, indptr, indices, q, k, v, bucket, table, scale, keep_sums)
+        return out if keep_sums else out[:2]
     graph, e = _rows_graph(row, indptr, indices)
-    return _bucket_forward(graph, e, q, k, v, bucket, table, scale)
+    return _bucket_forward(graph, e, q, k, v, bucket, table, scale, keep_sums)
 
 
-def attention_bucket_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, q, k, v, bucket, table, o, lse, d_o, scale):
-    """[dq, dk, dv, d_table] of attention_bucket_forward.  eid_t: for every position of the transposed CSR the position of
+def attention_bucket_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, q, k, v, bucket, table, sums, lse, d_o, scale):
+    """[dq, dk, dv, d_table] of attention_bucket_forward, with the sums it kept.  eid_t: for every position of the transposed CSR the position of
     the same edge in the row CSR."""
     graph, e = _both_graphs(row, indptr, indices, col, indptr_t, eid_t, indices_t)
-    return _bucket_backward(graph, e, q, k, v, bucket, table, o, lse, d_o, scale)
+    return _bucket_backward(graph, e, q, k, v, bucket, table, sums, lse, d_o, scale)
 
 
-def attention_bucket_forward_planned(plan, q, k, v, bucket, table, scale):
+def attention_bucket_forward_planned(plan, q, k, v, bucket, table, scale, keep_sums=False):
     """attention_bucket_forward on a plan of the row CSR."""
     native = native_functions_if_built()
     if native is not None:
-        return native.attention_bucket_forward_planned(plan.native(), q, k, v, bucket, table, scale)
+        out = native.attention_bucket_forward_planned(plan.native(), q, k, v, bucket, table, scale, keep_sums)
+        return out if keep_sums else out[:2]
     graph, e = _plan_rows(plan, q.size(0))
-    return _bucket_forward(graph, e, q, k, v, bucket, table, scale)
+    return _bucket_forward(graph, e, q, k, v, bucket, table, scale, keep_sums)
 
 
-def attention_bucket_backward_planned(plan_r, plan_t, q, k, v, bucket, table, o, lse, d_o, scale):
+def attention_bucket_backward_planned(plan_r, plan_t, q, k, v, bucket, table, sums, lse, d_o, scale):
     """attention_bucket_backward on plans of both orientations (plan_t with the transposed CSR's edge ids)."""
     graph, e = _plan_both(plan_r, plan_t, q.size(0), k.size(0))
-    return _bucket_backward(graph, e, q, k, v, bucket, table, o, lse, d_o, scale)
+    return _bucket_backward(graph, e, q, k, v, bucket, table, sums, lse, d_o, scale)
 
 
 def _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts):
@@ -966,7 +971,7 @@ def _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts):
     nb = _terms_bias(bucket, table, 2 * h, e, q.device)
     n = q.size(0)
     o = th.empty((n, h, 2 * d), dtype=q.dtype, device=q.device)
-    parts = th.empty((n, h, 2, 2 * d), dtype=q.dtype, device=q.device) if keep_parts else None
+    parts = th.empty((n, h, 2, 2 * d), dtype=_lse_dtype(q), device=q.device) if keep_parts else None
     lse = th.empty((n, 2 * h), dtype=_lse_dtype(q), device=q.device)
     _terms_call("attention_diff_forward", graph, elem, _capi.TERMS_DIFF_FWD, e, max(n, k.size(0)), h, d, nb, q.device,
                 [_p(q), _p(k), _p(v), _p(lam), _p(bucket), _p(table), nb, float(scale), _p(o), _p(parts), _p(lse)]
@@ -977,13 +982,13 @@ def _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts):
 def _diff_backward(graph, e, q, k, v, lam, parts, lse, d_o, scale, bucket, table):
     d_o = d_o.contiguous()
     _check_all(q=q, k=k, v=v, lam=lam, parts=parts, lse=lse, d_o=d_o)
-    elem = _elem(q, k, v, lam, parts, d_o, *([] if table is None else [table]))
+    elem = _elem(q, k, v, lam, d_o, *([] if table is None else [table]))
     _same_device(q, k, v, lam, parts, lse, d_o)
     h, d = _terms_shape(q, k, v, True)
     _terms_lam(lam, h)
     nb = _terms_bias(bucket, table, 2 * h, e, q.device)
     n = q.size(0)
-    if parts.shape != (n, h, 2, 2 * d) or d_o.shape != (n, h, 2 * d) or lse.shape != (n, 2 * h) or lse.dtype != _lse_dtype(q):
+    if parts.shape != (n, h, 2, 2 * d) or parts.dtype != _lse_dtype(q) or d_o.shape != (n, h, 2 * d) or lse.shape != (n, 2 * h) or lse.dtype != _lse_dtype(q):
         raise RuntimeError("parts, lse and d_o must have the forward's shapes and types")
     out = [th.empty_like(t) for t in (q, k, v, lam)] + ([th.empty_like(table)] if nb else [])
     _terms_call("attention_diff_backward", graph, elem, _capi.TERMS_DIFF_BWD, e, max(n, k.size(0)), h, d, nb, q.device,
@@ -995,8 +1000,8 @@ def _diff_backward(graph, e, q, k, v, lam, parts, lse, d_o, scale, bucket, table
 def attention_diff_forward(row, indptr, indices, q, k, v, lam, scale, bucket=None, table=None, keep_parts=True):
     """(o, lse, parts): differential attention, o = o1 - lam[h] * o2 with o1 and o2 the softmax sums of v under two maps of
     scores.  ``q`` (n, 2h, d) and ``k`` (m, 2h, d): heads 2i and 2i + 1 are the maps of head i of ``v`` (m, h, 2d);
-    ``lam`` (h,), of the same type; o (n, h, 2d), lse (n, 2h).  ``parts`` (n, h, 2, 2d), o1 and o2, is what the backward
-    reads (None without ``keep_parts``, for a call that has none).  ``bucket`` and ``table`` (buckets, 2h), both or neither: the
+    ``lam`` (h,), of the same type; o (n, h, 2d), lse (n, 2h).  ``parts`` (n, h, 2, 2d), o1 and o2 in lse's type, is what
+    the backward reads (None without ``keep_parts``, for a call that has none).  ``bucket`` and ``table`` (buckets, 2h), both or neither: the
     bias of attention_bucket_forward, a column per map, with the same rule for positions that take no part."""
     native = native_functions_if_built()
     if native is not None:

@@ -233,15 +233,15 @@ class GraphAttentionBucket(Function):
 
     @staticmethod
     def forward(ctx, row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, scale):
-        o, lse = _g.attention_bucket_forward(row, indptr, indices, Q, K, V, bucket, table, scale)
-        ctx.save_for_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, o, lse)
+        o, lse, sums = _g.attention_bucket_forward(row, indptr, indices, Q, K, V, bucket, table, scale, keep_sums=True)
+        ctx.save_for_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, sums, lse)
         ctx.scale = scale
         return o
 
     @staticmethod
     def backward(ctx, d_o):
-        graph, (Q, K, V, bucket, table, o, lse) = ctx.saved_tensors[:7], ctx.saved_tensors[7:]
-        dq, dk, dv, dt = _g.attention_bucket_backward(*graph, Q, K, V, bucket, table, o, lse, d_o, ctx.scale)
+        graph, (Q, K, V, bucket, table, sums, lse) = ctx.saved_tensors[:7], ctx.saved_tensors[7:]
+        dq, dk, dv, dt = _g.attention_bucket_backward(*graph, Q, K, V, bucket, table, sums, lse, d_o, ctx.scale)
         return None, None, None, None, None, None, None, dq, dk, dv, None, dt, None
 
 
@@ -259,8 +259,8 @@ class GraphAttentionBucketPlanned(Function):
 
     @staticmethod
     def forward(ctx, plan_r, plan_t, Q, K, V, bucket, table, scale):
-        o, lse = _g.attention_bucket_forward_planned(plan_r, Q, K, V, bucket, table, scale)
-        ctx.save_for_backward(Q, K, V, bucket, table, o, lse)
+        o, lse, sums = _g.attention_bucket_forward_planned(plan_r, Q, K, V, bucket, table, scale, keep_sums=True)
+        ctx.save_for_backward(Q, K, V, bucket, table, sums, lse)
         ctx.plans, ctx.scale = (plan_r, plan_t), scale
         return o
 

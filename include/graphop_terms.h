@@ -15,8 +15,10 @@
  *
  * Differential attention.  H pairs of maps: q (n_dst, 2H, D), k (n_src, 2H, D), v (n_src, H, 2D), lam (H); with n_buckets > 0 the
  * bias above with table (n_buckets, 2H), else bucket and table are null:
- *     o (n_dst, H, 2D) = o1 - lam[h] * o2, o1 and o2 the softmax sums of v under the maps 2h and 2h + 1
- *     parts (n_dst, H, 2, 2D): o1 and o2, what the backward reads; null where none follows;   lse (n_dst, 2H)
+ *     o (n_dst, H, 2D) = o1 - lam[h] * o2, o1 and o2 the softmax sums of v under the maps 2h and 2h + 1;   lse (n_dst, 2H)
+ *
+ * sums, for the backward (null where none follows): o before it is rounded, (n_dst, H, D), or o1 and o2, (n_dst, H, 2, 2D), as float
+ * (double for f64).  Without maps, and where the element type is float or double, o itself serves.
  *
  * Backward: the transposed CSR must carry eid_t (the row-CSR position of each of its positions); without it
  * GRAPHOP_ERR_INVALID_ARGUMENT.  Gradients of table and lam have the element type and are summed in 32 bits and more.
@@ -44,42 +46,43 @@ size_t graphop_terms_workspace_bytes(int op, int64_t n_edges, int64_t n_nodes, i
 #define GRAPHOP_DECLARE_TERMS(SUF, CT, I)                                                                                            \
   int graphop_attention_bucket_forward_##SUF(const I* row, const I* indptr, const I* indices, int64_t n_chunks, const CT* q,         \
                                              const CT* k, const CT* v, const int32_t* bucket, const CT* table, int n_buckets,        \
-                                             double scale, CT* o, void* lse, int64_t n_edges, int64_t n_dst, int64_t n_src, int H,   \
-                                             int D, void* workspace, size_t workspace_bytes, graphop_stream_t stream);               \
+                                             double scale, CT* o, void* sums, void* lse, int64_t n_edges, int64_t n_dst,             \
+                                             int64_t n_src, int H, int D, void* workspace, size_t workspace_bytes,                   \
+                                             graphop_stream_t stream);                                                               \
   int graphop_attention_bucket_backward_##SUF(                                                                                       \
       const I* row, const I* indptr, const I* indices, int64_t n_chunks, const I* col, const I* indptr_t, const I* eid_t,            \
       const I* indices_t, int64_t n_chunks_t, const CT* q, const CT* k, const CT* v, const int32_t* bucket, const CT* table,         \
-      int n_buckets, const CT* o, const void* lse, const CT* d_o, double scale, CT* dq, CT* dk, CT* dv, CT* d_table,                 \
+      int n_buckets, const void* sums, const void* lse, const CT* d_o, double scale, CT* dq, CT* dk, CT* dv, CT* d_table,                 \
       int64_t n_edges, int64_t n_dst, int64_t n_src, int H, int D, void* workspace, size_t workspace_bytes,                          \
       graphop_stream_t stream);                                                                                                      \
   int graphop_attention_diff_forward_##SUF(const I* row, const I* indptr, const I* indices, int64_t n_chunks, const CT* q,           \
                                            const CT* k, const CT* v, const CT* lam, const int32_t* bucket, const CT* table,          \
-                                           int n_buckets, double scale, CT* o, CT* parts, void* lse, int64_t n_edges,                \
+                                           int n_buckets, double scale, CT* o, void* sums, void* lse, int64_t n_edges,                \
                                            int64_t n_dst, int64_t n_src, int H, int D, void* workspace, size_t workspace_bytes,      \
                                            graphop_stream_t stream);                                                                 \
   int graphop_attention_diff_backward_##SUF(                                                                                         \
       const I* row, const I* indptr, const I* indices, int64_t n_chunks, const I* col, const I* indptr_t, const I* eid_t,            \
       const I* indices_t, int64_t n_chunks_t, const CT* q, const CT* k, const CT* v, const CT* lam, const int32_t* bucket,           \
-      const CT* table, int n_buckets, const CT* parts, const void* lse, const CT* d_o, double scale, CT* dq, CT* dk, CT* dv,         \
+      const CT* table, int n_buckets, const void* sums, const void* lse, const CT* d_o, double scale, CT* dq, CT* dk, CT* dv,         \
       CT* d_lam, CT* d_table, int64_t n_edges, int64_t n_dst, int64_t n_src, int H, int D, void* workspace, size_t workspace_bytes,  \
       graphop_stream_t stream);
 
 #define GRAPHOP_DECLARE_TERMS_PLANNED(SUF, CT)                                                                                       \
   int graphop_attention_bucket_forward_planned_##SUF(const graphop_plan_t* plan, const CT* q, const CT* k, const CT* v,              \
                                                      const int32_t* bucket, const CT* table, int n_buckets, double scale, CT* o,     \
-                                                     void* lse, int64_t n_dst, int64_t n_src, int H, int D, void* workspace,         \
+                                                     void* sums, void* lse, int64_t n_dst, int64_t n_src, int H, int D, void* workspace,         \
                                                      size_t workspace_bytes, graphop_stream_t stream);                               \
   int graphop_attention_bucket_backward_planned_##SUF(                                                                               \
       const graphop_plan_t* plan_r, const graphop_plan_t* plan_t, const CT* q, const CT* k, const CT* v, const int32_t* bucket,      \
-      const CT* table, int n_buckets, const CT* o, const void* lse, const CT* d_o, double scale, CT* dq, CT* dk, CT* dv,             \
+      const CT* table, int n_buckets, const void* sums, const void* lse, const CT* d_o, double scale, CT* dq, CT* dk, CT* dv,             \
       CT* d_table, int64_t n_dst, int64_t n_src, int H, int D, void* workspace, size_t workspace_bytes, graphop_stream_t stream);    \
   int graphop_attention_diff_forward_planned_##SUF(const graphop_plan_t* plan, const CT* q, const CT* k, const CT* v,                \
                                                    const CT* lam, const int32_t* bucket, const CT* table, int n_buckets,             \
-                                                   double scale, CT* o, CT* parts, void* lse, int64_t n_dst, int64_t n_src, int H,   \
+                                                   double scale, CT* o, void* sums, void* lse, int64_t n_dst, int64_t n_src, int H,   \
                                                    int D, void* workspace, size_t workspace_bytes, graphop_stream_t stream);         \
   int graphop_attention_diff_backward_planned_##SUF(                                                                                 \
       const graphop_plan_t* plan_r, const graphop_plan_t* plan_t, const CT* q, const CT* k, const CT* v, const CT* lam,              \
-      const int32_t* bucket, const CT* table, int n_buckets, const CT* parts, const void* lse, const CT* d_o, double scale, CT* dq,  \
+      const int32_t* bucket, const CT* table, int n_buckets, const void* sums, const void* lse, const CT* d_o, double scale, CT* dq,  \
       CT* dk, CT* dv, CT* d_lam, CT* d_table, int64_t n_dst, int64_t n_src, int H, int D, void* workspace, size_t workspace_bytes,   \
       graphop_stream_t stream);
 

@@ -97,8 +97,9 @@ def bounds(r, q, k, v, scale, dtype, bucket=None, table=None, staged=0.0):
     """How far a kernel's outputs may be from ``attention``'s, by first-order error analysis.  Inputs are exact; sums are held
     in `acc` (float32, or float64 for float64 tensors) with unit roundoff a, in any order (a sum of t terms is off by at most a t
     times the sum of magnitudes); stored tensors of `dtype` are off by u of their value; 2^x by 2^-21 in float32 (the hardware's
-    2^-22, and its argument), 2^-51 in float64, and below the smallest normal number of `acc` it is zero; `staged`: the unit roundoff of the type in which probabilities and score gradients
-    enter the products, 0 where they do not leave the accumulator type."""
+    2^-22, and its argument), 2^-51 in float64, and below the smallest normal number of `acc` it is zero; `staged`: the unit roundoff
+    of the type in which probabilities and score gradients enter the products, 0 where they do not leave the accumulator type; the
+    table's gradient then sums score gradients cut to 16 bits of mantissa."""
     acc = th.float64 if dtype == th.float64 else th.float32
     u, a = th.finfo(dtype).eps / 2, th.finfo(acc).eps / 2
     x, tiny = 2.0 ** -51 if acc == th.float64 else 2.0 ** -21, 2 * th.finfo(acc).tiny   # of a weight and of the scaled sum it joins
@@ -119,7 +120,7 @@ def bounds(r, q, k, v, scale, dtype, bucket=None, table=None, staged=0.0):
     e_sum += a * (deg[:, None, None] + 4) * zeros(n, maps, D).index_add(0, dst, p[..., None] * r["per"].abs())
     signed = e_sum * r["sign"].abs()[:, None] + 2 * a * (r["sums"] * r["sign"][:, None]).abs()
     out["o"] = (signed if not diff else signed[:, 0::2] + signed[:, 1::2]) + u * r["o"].abs()
-    e_kept = e_sum + u * r["sums"].abs()        # what the backward reads of the sums
+    e_kept = e_sum + 2 * a * r["sums"].abs()        # what the backward reads of the sums: unrounded
     if diff:
         out["parts"] = e_kept.view(r["parts"].shape)
     if "dp" not in r:
@@ -145,7 +146,9 @@ def bounds(r, q, k, v, scale, dtype, bucket=None, table=None, staged=0.0):
         inside = (bucket >= 0) & (bucket < table.shape[0])
         b = bucket[inside].long()
         count = th.bincount(b, minlength=table.shape[0]).to(F64)[:, None]
-        out["d_table"] = add(table.shape, b, es_g[inside]) + a * (count + 8) * add(table.shape, b, gs[inside]) + u * r["d_table"].abs()
+        cut = 2.0 ** -15 if staged else 0.0
+        out["d_table"] = add(table.shape, b, (eg + cut * gs)[inside]) + a * (count + 8) * add(table.shape, b, gs[inside]) \
+            + u * r["d_table"].abs()
     return out
 
 

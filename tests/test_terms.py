@@ -145,7 +145,7 @@ def _forward_code(**change):
         a["o"], a["parts"], a["lse"], a["e"], a["n"], a["m"], a["h"], a["d"], a["ws"], a["wsb"], None)]
     got.append(lib.graphop_attention_bucket_forward_f32_i32(
         a["row"], a["indptr"], a["indices"], a["chunks"], a["q"], a["k"], a["v"], a["bucket"], a["table"], a["nb"], 1.0, a["o"],
-        a["lse"], a["e"], a["n"], a["m"], a["h"], a["d"], a["ws"], a["wsb"], None))
+        a["parts"], a["lse"], a["e"], a["n"], a["m"], a["h"], a["d"], a["ws"], a["wsb"], None))
     return got
 
 

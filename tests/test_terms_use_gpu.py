@@ -71,7 +71,7 @@ def test_a_stack_of_both_layers_trains():
     want = [out, *th.autograd.grad(out, want_leaves, up)]
     # float32 through two layers: a few hundred roundings of 2^-24 of the largest value on the way
     for a, b in zip(got, want):
-        assert float((a.cpu().double() - b).abs().max()) <= 1000 * 2.0 ** -24 * max(1.0, float(b.abs().max()))
+        assert float((a.detach().cpu().double() - b.detach()).abs().max()) <= 1000 * 2.0 ** -24 * max(1.0, float(b.detach().abs().max()))
 
 
 @pytest.mark.parametrize("diff", [False, True])
