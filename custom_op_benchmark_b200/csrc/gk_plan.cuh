@@ -61,8 +61,8 @@ __device__ __forceinline__ void band_positions(const int32_t* __restrict__ erow,
 // first neighbour per node, and the widest range of neighbours any tile of 128 consecutive nodes reaches
 __device__ __forceinline__ void band_tiles(const int32_t* __restrict__ other, const int32_t* __restrict__ first,
                                            const int32_t* __restrict__ deg, long long n_nodes,
-                                           int32_t* __restrict__ node_lo, BandVerdict* __restrict__ verdict,
-                                           unsigned block) {
+                                           int32_t* __restrict__ node_lo, int32_t* __restrict__ tile_lo,
+                                           BandVerdict* __restrict__ verdict, unsigned block) {
   __shared__ int s_lo[kBandTileRows / 32], s_hi[kBandTileRows / 32];
   const long long r = (long long)block * kBandTileRows + threadIdx.x;
   int lo = INT_MAX, hi = INT_MIN;
@@ -82,6 +82,7 @@ __device__ __forceinline__ void band_tiles(const int32_t* __restrict__ other, co
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kBandTileRows / 32; ++w) { lo = min(lo, s_lo[w]); hi = max(hi, s_hi[w]); }
+    tile_lo[block] = lo;
     const int span = hi >= lo ? hi - lo + 1 : 0;
     if (span > *(volatile const int*)&verdict->max_span) atomicMax(&verdict->max_span, span);
   }
@@ -136,8 +137,8 @@ template <int kThreads>
 __global__ void __launch_bounds__(kThreads)
 plan_shape_kernel(const int32_t* __restrict__ erow, const int32_t* __restrict__ other, long long E,
                   const int32_t* __restrict__ first, const int32_t* __restrict__ deg, long long n_nodes,
-                  int32_t* __restrict__ node_lo, BandVerdict* __restrict__ verdict, unsigned tiles) {
-  if (blockIdx.x < tiles) band_tiles(other, first, deg, n_nodes, node_lo, verdict, blockIdx.x);
+                  int32_t* __restrict__ node_lo, int32_t* __restrict__ tile_lo, BandVerdict* __restrict__ verdict, unsigned tiles) {
+  if (blockIdx.x < tiles) band_tiles(other, first, deg, n_nodes, node_lo, tile_lo, verdict, blockIdx.x);
   else band_positions(erow, other, E, first, verdict, blockIdx.x - tiles, gridDim.x - tiles);
 }
 
@@ -147,6 +148,7 @@ inline size_t plan_bytes(long long C, long long E, long long n_nodes, int index_
   b += align_up((size_t)(tile_count(E, n_nodes, tile_cost(E, n_nodes)) + 1) * 4);   // tile boundaries
   if (index_bytes == 8) b += 2 * align_up((size_t)E * 4);
   b += 3 * align_up((size_t)(n_nodes > 0 ? n_nodes : 1) * 4) + align_up(kSkewBits / 8);
+  b += align_up((size_t)(n_nodes / kBandTileRows + 1) * 4);
   return b + kAlign;
 }
 
@@ -165,6 +167,7 @@ inline int plan_build(const I* row, const I* indptr, const I* eid, const I* indi
   int32_t* first = (int32_t*)ar.take((size_t)(n_nodes > 0 ? n_nodes : 1) * 4);
   int32_t* deg = (int32_t*)ar.take((size_t)(n_nodes > 0 ? n_nodes : 1) * 4);
   int32_t* node_lo = (int32_t*)ar.take((size_t)(n_nodes > 0 ? n_nodes : 1) * 4);
+  int32_t* tile_lo = (int32_t*)ar.take((size_t)(n_nodes / kBandTileRows + 1) * 4);
   unsigned* seen = (unsigned*)ar.take(kSkewBits / 8);
   if (ar.overflow) return GRAPHOP_ERR_WORKSPACE;
   plan->n_chunks = C;
@@ -187,6 +190,7 @@ inline int plan_build(const I* row, const I* indptr, const I* eid, const I* indi
   plan->node_lo = node_lo;
   plan->node_deg = deg;
   plan->node_first = first;
+  plan->tile_lo = tile_lo;
   {
     const unsigned aligning = (unsigned)((g.n_tiles + 256) / 256 < 4096 ? (g.n_tiles + 256) / 256 : 4096);
     const unsigned ranging = n_nodes > 0 && C > 0 ? (unsigned)((C + 255) / 256 < 8192 ? (C + 255) / 256 : 8192) : 0;
@@ -199,7 +203,7 @@ inline int plan_build(const I* row, const I* indptr, const I* eid, const I* indi
     const unsigned tiles = (unsigned)((n_nodes + kBandTileRows - 1) / kBandTileRows);
     const long long rounds = (E + kBandTileRows - 1) / kBandTileRows;
     plan_shape_kernel<kBandTileRows><<<tiles + (unsigned)(rounds < 592 ? rounds : 592), kBandTileRows, 0, st>>>(
-        g.erow, g.other, E, first, deg, n_nodes, node_lo, verdict, tiles);
+        g.erow, g.other, E, first, deg, n_nodes, node_lo, tile_lo, verdict, tiles);
     GK_LAUNCHED("plan_shape");
   }
   const bool analysed = g.other && n_nodes > 0;

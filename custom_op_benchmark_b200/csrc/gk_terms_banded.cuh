@@ -58,48 +58,28 @@ __device__ __forceinline__ void band_reduce(int lo, int deg, int part, bool writ
 }
 
 // ids[tile][column / kC][row][column % kC], kC columns per thread of the tile's kernel.  eid: the transposed CSR's edge ids, or null.
-// One orientation; a launch takes both where the backward needs both (blockIdx.z).
 struct BandIds {
-  const int32_t *node_lo, *node_deg, *node_first, *eid;
+  const int32_t *node_lo, *node_deg, *node_first, *tile_lo, *eid;
   long long n;
   int pitch, per;        // per: kC
   unsigned char* ids;
 };
-// A warp per row, four columns per lane at a time.  Bound by its instructions (a select per element) and by the chain node - position
-// - (edge id -) bucket, which every warp goes through once; with one column per lane and step, 443 instructions per row, 4.2M edges
-// took 13 us.
-static __global__ void __launch_bounds__(256)
-band_ids_kernel(const __grid_constant__ BandIds a0, const __grid_constant__ BandIds a1, const int32_t* __restrict__ bucket, int buckets) {
-  const bool other = blockIdx.z != 0;
-  const int32_t *node_lo = other ? a1.node_lo : a0.node_lo, *node_deg = other ? a1.node_deg : a0.node_deg,
-                *node_first = other ? a1.node_first : a0.node_first, *eid = other ? a1.eid : a0.eid;
-  const long long n = other ? a1.n : a0.n;
-  const int pitch = other ? a1.pitch : a0.pitch, shift = (other ? a1.per : a0.per) == 32 ? 5 : 4;
-  __shared__ int s_min[4], s_top[4];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const long long r0 = (long long)blockIdx.x * kTileM;
-  if (r0 >= n) return;
-  const int row = blockIdx.y * 8 + warp;
-  const long long r = r0 + row;
+// A warp per row (`row` of tile `tile`), four columns per lane at a time.  Bound by its instructions (a select per element) and by the
+// chain node - position - (edge id -) bucket, which every warp goes through once; with one column per lane and step, 443 instructions
+// per row, 4.2M edges took 13 us.
+__device__ __forceinline__ void band_ids_row(const BandIds& a, long long tile, int row, const int32_t* __restrict__ bucket, int buckets) {
+  const int lane = threadIdx.x & 31, shift = a.per == 32 ? 5 : 4;
+  const long long r = tile * kTileM + row;
   int deg = 0, lo = 0, first = 0;
-  if (r < n) {
-    deg = node_deg[r];
-    lo = node_lo[r];
-    first = node_first[r];
+  const int kmin = __ldg(a.tile_lo + tile);
+  if (r < a.n) {
+    deg = __ldg(a.node_deg + r);
+    lo = __ldg(a.node_lo + r);
+    first = __ldg(a.node_first + r);
   }
-  if (warp < 4) {
-    int l = INT_MAX, d = 0;
-    if (r0 + tid < n) {
-      d = node_deg[r0 + tid];
-      l = d > 0 ? node_lo[r0 + tid] : INT_MAX;
-    }
-    band_reduce(l, d, warp, lane == 0, s_min, s_top);
-  }
-  __syncthreads();
-  const int kmin = min(min(s_min[0], s_min[1]), min(s_min[2], s_min[3]));
-  unsigned char* out = (other ? a1.ids : a0.ids) + (size_t)blockIdx.x * pitch * kTileM + (row << shift);
+  unsigned char* out = a.ids + (size_t)tile * a.pitch * kTileM + (row << shift);
   const int skip = deg > 0 ? lo - kmin : 0;              // columns before the row's first
-  const int32_t* src = eid ? eid : bucket;
+  const int32_t* src = a.eid ? a.eid : bucket;
   constexpr int kSteps = kSpan / 128;
   int b[kSteps][4];
 #pragma unroll
@@ -109,7 +89,7 @@ band_ids_kernel(const __grid_constant__ BandIds a0, const __grid_constant__ Band
 #pragma unroll
     for (int q = 0; q < 4; ++q) b[i][q] = (unsigned)(k + q) < (unsigned)deg ? __ldg(at + q) : -1;
   }
-  if (eid) {
+  if (a.eid) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
 #pragma unroll
@@ -122,8 +102,12 @@ band_ids_kernel(const __grid_constant__ BandIds a0, const __grid_constant__ Band
     unsigned w = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) w |= ((unsigned)b[i][q] < (unsigned)buckets ? (unsigned)b[i][q] : kNoPart) << (8 * q);
-    if (c < pitch) *reinterpret_cast<unsigned*>(out + ((size_t)(c >> shift) << (shift + 7)) + (c & ((1 << shift) - 1))) = w;
+    if (c < a.pitch) *reinterpret_cast<unsigned*>(out + ((size_t)(c >> shift) << (shift + 7)) + (c & ((1 << shift) - 1))) = w;
   }
+}
+static __global__ void __launch_bounds__(256)
+band_ids_kernel(const __grid_constant__ BandIds a, const int32_t* __restrict__ bucket, int buckets) {
+  band_ids_row(a, blockIdx.x, blockIdx.y * 8 + (threadIdx.x >> 5), bucket, buckets);
 }
 
 // 16 consecutive columns of N regions of this thread's tensor-memory lane in flight together, one wait for all.  The wait names
@@ -165,6 +149,14 @@ __device__ __forceinline__ void store16(__nv_bfloat16* dst, const float (&v)[16]
     for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
     *reinterpret_cast<uint4*>(dst + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+// 16 floats, whole sectors: the lanes of a warp write rows far apart
+__device__ __forceinline__ void store_sums16(float* dst, const float (&v)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 8)
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + j), "f"(v[j]), "f"(v[j + 1]), "f"(v[j + 2]),
+                 "f"(v[j + 3]), "f"(v[j + 4]), "f"(v[j + 5]), "f"(v[j + 6]), "f"(v[j + 7])
+                 : "memory");
 }
 __device__ __forceinline__ bool not_finite(const float (&v)[16]) {
   float t = 0.f;
@@ -413,9 +405,7 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           out[j] = m == 0 ? o[j] : fmaf(-lam, o[j], out[j]);
         }
         if (p.sums && r < p.n_own) {
-          float4* at = reinterpret_cast<float4*>(p.sums + (((long long)r * p.H + head) * kMaps + m) * kD + f0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) at[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          store_sums16(p.sums + (((long long)r * p.H + head) * kMaps + m) * kD + f0, o);
         }
       }
       if (r < p.n_own) store16(p.o + ((long long)r * p.H + head) * kD + f0, out);
@@ -748,47 +738,58 @@ terms_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   }
 }
 
-// What the tiles' rows need: (lse in base-2 units, dO . o) of every node and map, and dO . o2 for dlam.  Eight lanes per node and head.
-// A row of which nothing took part has no probabilities, whatever dO holds.
-template <int kMaps>
+// What the tiles need before they begin, in one launch: the ids of both orientations (blockIdx.z 0 and 1, with kBucket alone), and (lse in
+// base-2 units, dO . o) of every node and map, with dO . o2 for dlam, eight lanes per node and head.  A row of which nothing took part
+// has no probabilities, whatever dO holds.
+template <int kMaps, bool kBucket>
 __global__ void __launch_bounds__(256)
-band_stat_kernel(const float* __restrict__ sums, const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse, long long cells,
-                 float2* __restrict__ stat, float* __restrict__ t2) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
+band_prepare_kernel(const __grid_constant__ BandIds a0, const __grid_constant__ BandIds a1, const int32_t* __restrict__ bucket, int buckets,
+                    const float* __restrict__ sums, const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse, long long cells,
+                    float2* __restrict__ stat, float* __restrict__ t2) {
+  if constexpr (kBucket) {
+    if (blockIdx.z < 2) {
+      const BandIds& a = blockIdx.z ? a1 : a0;
+      if ((long long)blockIdx.x * kTileM < a.n) band_ids_row(a, blockIdx.x, blockIdx.y * 8 + (threadIdx.x >> 5), bucket, buckets);
+      return;
+    }
+  }
   const int part = threadIdx.x & 7;
-  const bool in = i < cells;
-  float d[kMaps];
+  const long long stride = (long long)gridDim.x * gridDim.y * 32;
+  for (long long i0 = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * 32; i0 < cells; i0 += stride) {
+    const long long i = i0 + (threadIdx.x >> 3);
+    const bool in = i < cells;
+    float d[kMaps];
 #pragma unroll
-  for (int m = 0; m < kMaps; ++m) d[m] = 0.f;
-  if (in) {
-    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(d_o + i * kD) + part);
-    const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv);
+    for (int m = 0; m < kMaps; ++m) d[m] = 0.f;
+    if (in) {
+      const uint4 gv = __ldg(reinterpret_cast<const uint4*>(d_o + i * kD) + part);
+      const __nv_bfloat162* g2 = reinterpret_cast<const __nv_bfloat162*>(&gv);
+#pragma unroll
+      for (int m = 0; m < kMaps; ++m) {
+        const float4* at = reinterpret_cast<const float4*>(sums + (i * kMaps + m) * kD) + 2 * part;
+        const float4 x = __ldg(at), y = __ldg(at + 1);
+        const float of[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 gf = __bfloat1622float2(g2[e]);
+          d[m] += of[2 * e] * gf.x + of[2 * e + 1] * gf.y;
+        }
+      }
+    }
 #pragma unroll
     for (int m = 0; m < kMaps; ++m) {
-      const float4* at = reinterpret_cast<const float4*>(sums + (i * kMaps + m) * kD) + 2 * part;
-      const float4 x = __ldg(at), y = __ldg(at + 1);
-      const float of[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 gf = __bfloat1622float2(g2[e]);
-        d[m] += of[2 * e] * gf.x + of[2 * e + 1] * gf.y;
+      for (int o = 1; o < 8; o <<= 1) d[m] += __shfl_xor_sync(kFull, d[m], o);
+      if (in && part == 0) {
+        const float l = lse[i * kMaps + m];
+        const bool none = l == -INFINITY;
+        if (none) d[m] = 0.f;
+        stat[i * kMaps + m] = make_float2(none ? INFINITY : l * (float)kLog2e, d[m]);
+        if (m == 1) t2[i] = d[m];
       }
     }
   }
-#pragma unroll
-  for (int m = 0; m < kMaps; ++m) {
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) d[m] += __shfl_xor_sync(kFull, d[m], o);
-    if (in && part == 0) {
-      const float l = lse[i * kMaps + m];
-      const bool none = l == -INFINITY;
-      if (none) d[m] = 0.f;
-      stat[i * kMaps + m] = make_float2(none ? INFINITY : l * (float)kLog2e, d[m]);
-      if (m == 1) t2[i] = d[m];
-    }
-  }
 }
-
 
 // ---------------------------------------------------------------------------------------------------------
 // tiles done again, edge by edge: kSide 0 forward, 1 destination side (dq), 2 source side (dk, dv)
@@ -1000,17 +1001,10 @@ inline int band_pitch(const graphop_plan_t* plan) { return (plan->band_span + kK
 inline long long band_tiles_of(long long n) { return (n + kTileM - 1) / kTileM; }
 inline bool band_plan_ok(const graphop_plan_t* plan, long long n, int H) {
   return (plan->flags & GRAPHOP_PLAN_DENSE_BAND) && plan->band_span > 0 && plan->band_span <= kSpan && plan->node_lo && plan->node_deg &&
-         plan->node_first && n >= 1 && n <= plan->n_nodes && H <= 65535;
+         plan->node_first && plan->tile_lo && n >= 1 && n <= plan->n_nodes && H <= 65535;
 }
 inline BandIds band_ids_of(const graphop_plan_t* plan, const int32_t* eid, long long n, int per, unsigned char* ids) {
-  return BandIds{plan->node_lo, plan->node_deg, plan->node_first, eid, n, band_pitch(plan), per, ids};
-}
-// a1: null, or the other orientation
-inline int run_band_ids(const BandIds& a0, const BandIds* a1, const int32_t* bucket, int buckets, cudaStream_t st) {
-  const long long tiles = band_tiles_of(a1 && a1->n > a0.n ? a1->n : a0.n);
-  band_ids_kernel<<<dim3((unsigned)tiles, kTileM / 8, a1 ? 2 : 1), 256, 0, st>>>(a0, a1 ? *a1 : a0, bucket, buckets);
-  GK_LAUNCHED("band_ids");
-  return GRAPHOP_OK;
+  return BandIds{plan->node_lo, plan->node_deg, plan->node_first, plan->tile_lo, eid, n, band_pitch(plan), per, ids};
 }
 template <int kSide, int kMaps, bool kBucket>
 inline int run_band_again(const AgainArgs& a, cudaStream_t st) {
@@ -1035,7 +1029,11 @@ inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat
     return GRAPHOP_ERR_UNSUPPORTED;
   static std::atomic<bool> configured[64];
   GK_TRY(allow_smem(terms_forward_kernel<kMaps, kBucket>, L::kBytes, configured));
-  if (kBucket) GK_TRY(run_band_ids(band_ids_of(plan, nullptr, c.n_dst, 32, const_cast<unsigned char*>(t.ids)), nullptr, c.bucket, c.buckets, st));
+  if (kBucket) {
+    band_ids_kernel<<<dim3((unsigned)tiles, kTileM / 8), 256, 0, st>>>(
+        band_ids_of(plan, nullptr, c.n_dst, 32, const_cast<unsigned char*>(t.ids)), c.bucket, c.buckets);
+    GK_LAUNCHED("band_ids");
+  }
   t.table = c.table; t.lam = c.lam; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan->node_lo; t.node_deg = plan->node_deg;
   t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.o = o; t.sums = (float*)sums; t.lse = (float*)lse;
   terms_forward_kernel<kMaps, kBucket><<<dim3((unsigned)tiles, (unsigned)c.H), kThreads, L::kBytes, st>>>(mq, mk, mv, t);
@@ -1080,13 +1078,10 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   constexpr int smem = LD::kBytes > LS::kBytes ? LD::kBytes : LS::kBytes;
   static std::atomic<bool> configured[64];
   GK_TRY(allow_smem(terms_backward_kernel<kMaps, kBucket>, smem, configured));
-  if (kBucket) {
-    const BandIds other = band_ids_of(plan_t, plan_t->eid, c.n_src, LS::kC, ids_t);
-    GK_TRY(run_band_ids(band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, ids), &other, c.bucket, c.buckets, st));
-  }
-  const long long cells = c.n_dst * c.H;
-  band_stat_kernel<kMaps><<<(unsigned)((cells * 8 + 255) / 256), 256, 0, st>>>((const float*)sums, dout, (const float*)lse, cells, t.stat, t2);
-  GK_LAUNCHED("band_stat");
+  const BandIds own = band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, ids), other = band_ids_of(plan_t, plan_t->eid, c.n_src, LS::kC, ids_t);
+  band_prepare_kernel<kMaps, kBucket><<<dim3((unsigned)(kBucket && tiles_t > tiles ? tiles_t : tiles), kTileM / 8, kBucket ? 3 : 1), 256, 0, st>>>(
+      own, other, c.bucket, c.buckets, (const float*)sums, dout, (const float*)lse, c.n_dst * c.H, t.stat, t2);
+  GK_LAUNCHED("band_prepare");
   t.table = c.table; t.lam = c.lam; t.ids = ids; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan_r->node_lo;
   t.node_deg = plan_r->node_deg; t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.out0 = dq;
   TermsTile u = t;
@@ -1110,7 +1105,8 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
 template <>
 inline int banded_terms_forward<__nv_bfloat16>(const graphop_plan_t* plan, const TermsCall<__nv_bfloat16>& c, __nv_bfloat16* o,
                                                void* sums, void* lse, void* ws, size_t wsb, cudaStream_t st) {
-  if (c.row_d() != banded::kD || c.buckets > banded::kMostBandBuckets || c.n_src < 1 || !banded::band_plan_ok(plan, c.n_dst, c.H))
+  if (c.row_d() != banded::kD || c.buckets > banded::kMostBandBuckets || c.n_src < 1 || !banded::band_plan_ok(plan, c.n_dst, c.H) ||
+      ((uintptr_t)sums & 31))   // store_sums16's alignment
     return GRAPHOP_ERR_UNSUPPORTED;
   Arena ar(ws, wsb);
   if (!c.diff) return banded::terms_forward<1, true>(plan, c, o, sums, lse, ar, st);

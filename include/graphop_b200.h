@@ -185,6 +185,7 @@ typedef struct graphop_plan {
   int32_t tile;            /* cost per work tile the boundaries were made for */
   int32_t gather_repeats;  /* of up to 1024 evenly spaced positions, how many gather a row that another one gathers */
   const int32_t* node_first; /* device, n_nodes: first position of every node that owns any */
+  const int32_t* tile_lo;    /* device: first neighbour of any of 128 consecutive nodes, INT_MAX where none has one (as node_lo) */
 } graphop_plan_t;
 
 /* Bytes of device memory (256-byte aligned) a plan of these sizes needs. */
