@@ -190,10 +190,17 @@ __device__ __forceinline__ unsigned id_at(const uint4& w, int j) {
   return (x >> (8 * (j & 3))) & 255u;
 }
 
+// Two maps: the output is the difference of two sums, and probabilities rounded to bfloat16 would be the larger part of its error
+// (0.0025 against 0.0017 of the rounded output alone), so that a second product adds what the rounding left off, rounded again: 16 bits
+// of mantissa.  The room for it comes from k, which needs no second slot: block b + 1 is asked for at the same moment either way,
+// when the scores of b are there.  One map keeps one product: three tiles share an SM.
 template <int kMaps>
 struct FwdLayout {
-  static constexpr int kOffP = kOffK + kSlots * 2 * kBandBytes;           // a staging tile per map
-  static constexpr int kOffBar = kOffP + kMaps * kBlockBytes;
+  static constexpr bool kRest = kMaps == 2;                               // probabilities in two parts
+  static constexpr int kOffV = kOffK + kBandBytes;                        // of slot 0
+  static constexpr int kStepK = kRest ? 0 : 2 * kBandBytes, kStepV = kRest ? kBandBytes : 2 * kBandBytes;   // from slot 0 to slot 1
+  static constexpr int kOffP = kOffK + (kRest ? 3 : 4) * kBandBytes;      // a staging tile per map and part
+  static constexpr int kOffBar = kOffP + (kRest ? 2 : 1) * kMaps * kBlockBytes;
   static constexpr int kOffRed = kOffBar + 128;                           // maxima, and at the end sums, of the two column groups
   static constexpr int kOffTable = kOffRed + kMaps * kColGroups * kTileM * 4;
   static constexpr int kBytes = kOffTable + kMaps * 256 * 4 + 1024;
@@ -251,15 +258,15 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     int nb = (ktop - kmin) / kKeys + 1;
     nb = nb < p.pitch / kKeys ? nb : p.pitch / kKeys;
     auto issue_band = [&](int b) {   // one thread
-      const uint32_t bar = bar_full + 8 * (b & 1), at = s_base + kOffK + (b & 1) * 2 * kBandBytes;
+      const uint32_t bar = bar_full + 8 * (b & 1);
       mbar_expect_tx(bar, (uint32_t)(2 * kBandBytes));
-      tma_load_3d(at, &map_k, bar, 0, head, kmin + b * kKeys);
-      tma_load_3d(at + kBandBytes, &map_v, bar, 0, head, kmin + b * kKeys);
+      tma_load_3d(s_base + kOffK + (b & 1) * L::kStepK, &map_k, bar, 0, head, kmin + b * kKeys);
+      tma_load_3d(s_base + L::kOffV + (b & 1) * L::kStepV, &map_v, bar, 0, head, kmin + b * kKeys);
     };
     constexpr int kSteps = kD / kMaps / 16;   // of 16 features, per map
     auto issue_scores = [&](int b) {   // one thread
       constexpr uint32_t idesc = umma_idesc(kTileM, kKeys, false);
-      const uint32_t at = s_base + kOffK + (b & 1) * 2 * kBandBytes;
+      const uint32_t at = s_base + kOffK + (b & 1) * L::kStepK;
 #pragma unroll
       for (int kk = 0; kk < kD / 16; ++kk)
         umma_f16(tmem + (kk / kSteps) * kKeys, umma_desc(s_base + kOffQ + kk * 32, 16, 1024), umma_desc(at + kk * 32, 16, 1024), idesc,
@@ -270,9 +277,9 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       tma_load_3d(s_base + kOffQ, &map_q, bar_load, 0, head, (int)r0);
       tma_load_3d(s_base + kOffQ + kBandBytes, &map_q, bar_load, 0, head, (int)r0 + kKeys);
       issue_band(0);
-      if (nb > 1) issue_band(1);
+      if (!L::kRest && nb > 1) issue_band(1);
     }
-    int issued = nb < kSlots ? nb : kSlots;
+    int issued = L::kRest || nb < kSlots ? 1 : kSlots;
     bool ok = __syncthreads_and(mbar_wait(bar_load, 0) && mbar_wait(bar_full, 0));
 
     const int jlo = deg > 0 ? lo - kmin : 1, jhi = deg > 0 ? lo - kmin + deg - 1 : 0;   // this row's columns of the band
@@ -306,7 +313,7 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       ok = __syncthreads_and(ok && mbar_wait(bar_s, b & 1));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (ok && b > 0 && b + 1 < nb) {   // block b - 1's slot is free
+      if (ok && (b > 0 || L::kRest) && b + 1 < nb) {   // block b - 1's slot is free, and where k has one alone, b's too
         if (tid == 0) issue_band(b + 1);
         issued = b + 2;
       }
@@ -347,7 +354,7 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const float ref = mx[m] == -INFINITY ? 0.f : mx[m];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t packed[8];
+          uint32_t packed[8], rest[8];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             float p0 = 0.f, p1 = 0.f;
@@ -357,8 +364,11 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
               l[m] += p0 + p1;
             }
             packed[j / 2] = pack_bf16(p0, p1);
+            if constexpr (L::kRest)
+              rest[j / 2] = pack_bf16(p0 - __uint_as_float(packed[j / 2] << 16), p1 - __uint_as_float(packed[j / 2] & 0xffff0000u));
           }
           stage16(prow + m * kBlockBytes, row, cg * 4 + 2 * half, packed);
+          if constexpr (L::kRest) stage16(prow + (kMaps + m) * kBlockBytes, row, cg * 4 + 2 * half, rest);
         }
       }
       // the probabilities were written through the generic proxy; the tensor core reads through the async proxy
@@ -368,13 +378,15 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (ok && tid == 0) {
         constexpr uint32_t idesc = umma_idesc(kTileM, kD, true);
-        const uint32_t at = s_base + kOffK + (b & 1) * 2 * kBandBytes + kBandBytes;
+        const uint32_t at = s_base + L::kOffV + (b & 1) * L::kStepV;
 #pragma unroll
-        for (int m = 0; m < kMaps; ++m)
+        for (int part = 0; part < (L::kRest ? 2 : 1); ++part)
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            umma_f16(tmem + (kMaps + m) * kKeys, umma_desc(s_base + L::kOffP + m * kBlockBytes + ks * 32, 16, 1024),
-                     umma_desc(at + ks * 16 * kRowBytes, 16, 1024), idesc, (b | ks) != 0);
+          for (int m = 0; m < kMaps; ++m)
+#pragma unroll
+            for (int ks = 0; ks < kKeys / 16; ++ks)
+              umma_f16(tmem + (kMaps + m) * kKeys, umma_desc(s_base + L::kOffP + (part * kMaps + m) * kBlockBytes + ks * 32, 16, 1024),
+                       umma_desc(at + ks * 16 * kRowBytes, 16, 1024), idesc, (part | b | ks) != 0);
         if (b + 1 < nb) issue_scores(b + 1);
         umma_commit(bar_s);
       }
