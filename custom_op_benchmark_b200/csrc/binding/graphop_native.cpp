@@ -825,7 +825,9 @@ Result terms_on_tables(std::initializer_list<Tensor> index, const TermsInputs& x
 }
 Result terms_on_plans(const PlanHandle& plan_r, const PlanHandle& plan_t, const TermsInputs& x, bool diff, double scale) {
   if (left_to_python({&x.q, &x.k, &x.v, &x.lam, &x.bucket, &x.table})) return c10::nullopt;
-  check_terms_plan(plan_r, x.q.defined() && x.q.dim() ? x.q.size(0) : 0);
+  const auto rows_of = [](const Tensor& t) { return t.defined() && t.dim() ? t.size(0) : 0; };
+  check_terms_plan(plan_r, rows_of(x.q));
+  if (rows_of(x.k) < plan_t.graph->plan.n_nodes) fail("q and k must have a row for each of the plans' nodes");
   TermsGraph graph;
   graph.rows = plan_r.graph;
   graph.cols = plan_t.graph;

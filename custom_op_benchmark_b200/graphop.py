@@ -878,9 +878,13 @@ def _plan_rows(plan, n_dst):
     return (None, 4, [plan.ref()]), plan.n_edges
 
 
-def _plan_both(plan_r, plan_t, n_dst, n_src):
+def check_plan_rows(plan_r, plan_t, n_dst, n_src):
     if n_dst < plan_r.n_nodes or n_src < plan_t.n_nodes:
         raise RuntimeError("q and k must have a row for each of the plans' nodes")
+
+
+def _plan_both(plan_r, plan_t, n_dst, n_src):
+    check_plan_rows(plan_r, plan_t, n_dst, n_src)
     if plan_t.n_edges != plan_r.n_edges:
         raise RuntimeError("the plans disagree on the number of edges")
     if plan_r.n_edges and not plan_t.c.eid:

@@ -259,6 +259,7 @@ class GraphAttentionBucketPlanned(Function):
 
     @staticmethod
     def forward(ctx, plan_r, plan_t, Q, K, V, bucket, table, scale):
+        _g.check_plan_rows(plan_r, plan_t, Q.size(0), K.size(0))
         o, lse, sums = _g.attention_bucket_forward_planned(plan_r, Q, K, V, bucket, table, scale, keep_sums=True)
         ctx.save_for_backward(Q, K, V, bucket, table, sums, lse)
         ctx.plans, ctx.scale = (plan_r, plan_t), scale
@@ -309,6 +310,7 @@ class GraphAttentionDiffPlanned(Function):
 
     @staticmethod
     def forward(ctx, plan_r, plan_t, Q, K, V, lam, scale, bucket=None, table=None):
+        _g.check_plan_rows(plan_r, plan_t, Q.size(0), K.size(0))
         o, lse, parts = _g.attention_diff_forward_planned(plan_r, Q, K, V, lam, scale, bucket, table,
                                                           keep_parts=any(ctx.needs_input_grad))
         ctx.save_for_backward(Q, K, V, lam, parts, lse, bucket, table)

@@ -311,3 +311,19 @@ def test_refusals():
             graphop.relative_buckets_planned(plan_r, 32, 128, True, pos, None)
     with pytest.raises(RuntimeError, match="index type"):
         graphop.relative_buckets(*graph, 32, 128, True, th.zeros(64, dtype=th.int64, device=DEV), None)
+
+
+def test_a_plan_that_names_more_sources_than_there_are_rows_is_refused():
+    """Before the forward reads them, with and without the compiled nodes."""
+    layer = Layer(ZOO[0][1], True, 7, 4, 32, th.float32)
+    q, k, v, lam = (t.to(DEV) for t in (layer.q, layer.k, layer.v, layer.lam))
+    bucket, table = layer.terms()
+    plans = layer.plans()
+    short = [k[:-1].contiguous(), v[:-1].contiguous()]
+    bias = [bucket, table[:, :4].contiguous()]
+    calls = [lambda f: f(*plans, q, *short, lam, 1.0, bucket, table),
+             lambda f: f(*plans, v, short[1], short[1], *bias, 1.0)]
+    for cls, call in zip((wrapper.GraphAttentionDiffPlanned, wrapper.GraphAttentionBucketPlanned), calls):
+        for apply in (cls.apply, super(cls, cls).apply):
+            with pytest.raises(RuntimeError, match="a row for each of the plan"):
+                call(apply)
