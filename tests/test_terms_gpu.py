@@ -327,3 +327,18 @@ def test_a_plan_that_names_more_sources_than_there_are_rows_is_refused():
         for apply in (cls.apply, super(cls, cls).apply):
             with pytest.raises(RuntimeError, match="a row for each of the plan"):
                 call(apply)
+
+
+@pytest.mark.parametrize("both,reach,last", [(False, 3865, 1023), (False, 3870, 1024), (False, 3874, 1025), (True, 23103, 1023),
+                                             (True, 23137, 1024), (True, 23171, 1025)])
+def test_limits_around_the_table_by_distance(both, reach, last):
+    """Limits that end at 1024 or before make a table of the distances, others are searched; distances on both sides of the last one."""
+    assert graphop.bucket_limits(5 if both else 10, reach)[-1] == last
+    n = 2300
+    at = th.arange(n) * (1 - 2 * (th.arange(n) % 2)) if both else -th.arange(n)
+    graph = [th.zeros(1, dtype=th.int64, device=DEV), th.tensor([0, n], device=DEV), th.arange(n, device=DEV)]
+    zero = th.zeros(1, dtype=th.int64)
+    want = ref.relative_buckets(th.zeros(n, dtype=th.int64), th.arange(n), 10, reach, both, zero, at)
+    assert th.equal(graphop.relative_buckets(*graph, 10, reach, both, zero.to(DEV), at.to(DEV)).cpu(), want)
+    plan = graphop.GraphPlan(graph[0], graph[1], None, graph[2], 1)
+    assert th.equal(graphop.relative_buckets_planned(plan, 10, reach, both, zero.to(DEV), at.to(DEV)).cpu(), want)
