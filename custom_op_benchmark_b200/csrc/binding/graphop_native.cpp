@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <cstring>
 #include <limits>
 #include <memory>
 #include <mutex>
@@ -907,7 +908,13 @@ c10::optional<at::ScalarType> check_positions(const Tensor& dst, const Tensor& s
   }
   return type;
 }
-Tensor relative_buckets_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const std::vector<int64_t>& limits, bool both,
+// limits: 64-bit numbers, packed
+std::vector<int64_t> unpacked(const std::string& limits) {
+  std::vector<int64_t> at(limits.size() / 8);
+  if (!at.empty()) std::memcpy(at.data(), limits.data(), at.size() * 8);
+  return at;
+}
+Tensor relative_buckets_(const Tensor& row, const Tensor& indptr, const Tensor& indices, const std::string& limits, bool both,
                          const Later& dst_in, const Later& src_in) {
   const Tensor dst = given(dst_in), src = given(src_in);
   check_input(row, "row"); check_input(indptr, "indptr"); check_input(indices, "indices");
@@ -915,27 +922,29 @@ Tensor relative_buckets_(const Tensor& row, const Tensor& indptr, const Tensor& 
   check_chunks(row, indptr);
   check_positions(dst, src, -1, indices.scalar_type(), indices.device());
   Call c(indices);
+  const std::vector<int64_t> limit = unpacked(limits);
   Tensor out = at::empty({indices.size(0)}, indices.options().dtype(at::kInt));
   const auto call = [&](auto* i, auto&& f) {
     using I = std::remove_pointer_t<decltype(i)>;
     return f(owners<I>(row, indptr), (const I*)ptr<I>(indptr), (const I*)ptr<I>(indices), row.size(0), (const I*)ptr<I>(dst),
-             (const I*)ptr<I>(src), limits.data(), (int)limits.size(), (int)both, out.data_ptr<int32_t>(), indices.size(0), raw(c.stream));
+             (const I*)ptr<I>(src), limit.data(), (int)limit.size(), (int)both, out.data_ptr<int32_t>(), indices.size(0), raw(c.stream));
   };
   check_status(ib == 8 ? call((int64_t*)nullptr, graphop_relative_buckets_i64) : call((int32_t*)nullptr, graphop_relative_buckets_i32),
                "relative_buckets");
   return out;
 }
-Tensor relative_buckets_plan(const PlanHandle& plan, const std::vector<int64_t>& limits, bool both, const Later& dst_in, const Later& src_in,
+Tensor relative_buckets_plan(const PlanHandle& plan, const std::string& limits, bool both, const Later& dst_in, const Later& src_in,
                              const Tensor& like) {
   const Tensor dst = given(dst_in), src = given(src_in);
   const graphop_plan_t* p = &plan.graph->plan;
   const auto type = check_positions(dst, src, p->n_nodes, c10::nullopt, like.device());
   Call c(like);
+  const std::vector<int64_t> limit = unpacked(limits);
   Tensor out = at::empty({p->n_edges}, like.options().dtype(at::kInt));
   int32_t* to = out.data_ptr<int32_t>();
-  check_status(type == at::kLong ? graphop_relative_buckets_planned_i64(p, ptr<int64_t>(dst), ptr<int64_t>(src), limits.data(), (int)limits.size(),
+  check_status(type == at::kLong ? graphop_relative_buckets_planned_i64(p, ptr<int64_t>(dst), ptr<int64_t>(src), limit.data(), (int)limit.size(),
                                                                         (int)both, to, raw(c.stream))
-                                 : graphop_relative_buckets_planned_i32(p, ptr<int32_t>(dst), ptr<int32_t>(src), limits.data(), (int)limits.size(),
+                                 : graphop_relative_buckets_planned_i32(p, ptr<int32_t>(dst), ptr<int32_t>(src), limit.data(), (int)limit.size(),
                                                                         (int)both, to, raw(c.stream)),
                "relative_buckets_planned");
   return out;

@@ -15,6 +15,7 @@ and float64; ``dy`` is made contiguous instead of being read unchecked
 """
 import collections
 import functools
+import struct
 
 import torch as th
 
@@ -727,16 +728,16 @@ def bucket_limits(num_buckets, max_distance):
 
 
 def _limits(num_buckets, max_distance, bidirectional):
-    import ctypes
+    """The limits of a direction as the library takes them, packed once: a conversion of hundreds of them costs more than the call."""
     if bidirectional and num_buckets % 2:
         raise ValueError("num_buckets must be even for both directions")
-    at = _limits_of(int(num_buckets) // 2 if bidirectional else int(num_buckets), int(max_distance))
-    return at, (ctypes.c_int64 * len(at))(*at)
+    return _limits_of(int(num_buckets) // 2 if bidirectional else int(num_buckets), int(max_distance))
 
 
 @functools.lru_cache(maxsize=64)
 def _limits_of(num_buckets, max_distance):
-    return tuple(bucket_limits(num_buckets, max_distance))
+    at = bucket_limits(num_buckets, max_distance)
+    return struct.pack("=%dq" % len(at), *at)
 
 
 def _positions(dst_pos, src_pos, n_dst, n_src, dtype, device):
@@ -762,10 +763,10 @@ def relative_buckets(row, indptr, indices, num_buckets, max_distance, bidirectio
     without it all are for positions behind, and those ahead share bucket 0.  Within a direction the distances are
     shared out as ``bucket_limits`` says.  ``dst_pos`` and ``src_pos`` (index type) default to the node ids; every
     node that an edge names needs a position."""
-    at, limits = _limits(num_buckets, max_distance, bidirectional)
+    limits = _limits(num_buckets, max_distance, bidirectional)
     native = native_functions_if_built()
     if native is not None:
-        return native.relative_buckets(row, indptr, indices, at, bool(bidirectional), dst_pos, src_pos)
+        return native.relative_buckets(row, indptr, indices, limits, bool(bidirectional), dst_pos, src_pos)
     _check_all(row=row, indptr=indptr, indices=indices)
     index = _index(row, indptr, indices)
     e, c = indices.size(0), _chunks(row, indptr)
@@ -773,23 +774,23 @@ def relative_buckets(row, indptr, indices, num_buckets, max_distance, bidirectio
     out = th.empty(e, dtype=th.int32, device=indices.device)
     with th.cuda.device(out.device):
         _check(getattr(_capi.lib(), "graphop_relative_buckets_" + index[0])(
-            _owners(row, indptr), _p(indptr), _p(indices), c, _p(dst_pos), _p(src_pos), limits, len(at), int(bool(bidirectional)), _p(out), e,
+            _owners(row, indptr), _p(indptr), _p(indices), c, _p(dst_pos), _p(src_pos), limits, len(limits) // 8, int(bool(bidirectional)), _p(out), e,
             th.cuda.current_stream(out.device).cuda_stream), "relative_buckets")
     return out
 
 
 def relative_buckets_planned(plan, num_buckets, max_distance, bidirectional=True, dst_pos=None, src_pos=None):
     """relative_buckets on a plan of the row CSR; the positions are int32 or int64, both the same."""
-    at, limits = _limits(num_buckets, max_distance, bidirectional)
+    limits = _limits(num_buckets, max_distance, bidirectional)
     native = native_functions_if_built()
     if native is not None:
-        return native.relative_buckets_planned(plan.native(), at, bool(bidirectional), dst_pos, src_pos, plan._memory)
+        return native.relative_buckets_planned(plan.native(), limits, bool(bidirectional), dst_pos, src_pos, plan._memory)
     dtype = _positions(dst_pos, src_pos, plan.n_nodes, None, None, plan.device)
     out = th.empty(plan.n_edges, dtype=th.int32, device=plan.device)
     suffix = "i64" if dtype == th.int64 else "i32"
     with th.cuda.device(out.device):
         _check(getattr(_capi.lib(), "graphop_relative_buckets_planned_" + suffix)(
-            plan.ref(), _p(dst_pos), _p(src_pos), limits, len(at), int(bool(bidirectional)), _p(out),
+            plan.ref(), _p(dst_pos), _p(src_pos), limits, len(limits) // 8, int(bool(bidirectional)), _p(out),
             th.cuda.current_stream(out.device).cuda_stream), "relative_buckets_planned")
     return out
 
