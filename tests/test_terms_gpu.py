@@ -342,3 +342,48 @@ def test_limits_around_the_table_by_distance(both, reach, last):
     assert th.equal(graphop.relative_buckets(*graph, 10, reach, both, zero.to(DEV), at.to(DEV)).cpu(), want)
     plan = graphop.GraphPlan(graph[0], graph[1], None, graph[2], 1)
     assert th.equal(graphop.relative_buckets_planned(plan, 10, reach, both, zero.to(DEV), at.to(DEV)).cpu(), want)
+
+
+@pytest.mark.parametrize("diff,buckets", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("name", ["zoo", "band"])
+def test_more_rows_than_the_graph_names(diff, buckets, name):
+    """A padded batch: node rows behind the last one of a plan or of a chunk table come out as zeros, whatever they hold."""
+    g = ZOO[2][1] if name == "zoo" else graphs.banded_graph(1, 300, 60)
+    d = 64 if not diff else 32
+    layer = Layer(g, diff, buckets, 2, d, th.bfloat16, seed=21)
+    plans = layer.plans()
+    for on in (None, plans):
+        want = layer.step(on)
+        x = [t.to(DEV) for t in (layer.q, layer.k, layer.v, layer.lam, layer.table) if t is not None]
+        pad = [th.full((5, *t.shape[1:]), math.nan, dtype=t.dtype, device=DEV) for t in x[:3]]
+        leaves = [th.cat([t, p]).requires_grad_(True) for t, p in zip(x[:3], pad)] + [t.requires_grad_(True) for t in x[3:]]
+        d_o, layer.d_o = layer.d_o, th.cat([layer.d_o, th.zeros(5, *layer.d_o.shape[1:], dtype=layer.dt)])
+        got = layer.step(on, leaves)
+        layer.d_o = d_o
+        for n, w, t in zip(layer.names(), want, got):
+            if t.shape != w.shape:
+                assert bool((t[len(w):] == 0).all()), n
+                t = t[: len(w)]
+            assert not bool(th.isnan(t).any()), n
+        layer.check([t[: len(w)] for t, w in zip(got, want)], th.finfo(th.bfloat16).eps / 2 if name == "band" else 0.0)
+
+
+@pytest.mark.parametrize("diff,buckets", KINDS[::2], ids=KIND_IDS[::2])
+def test_ids_and_biases_at_odd_addresses(diff, buckets):
+    """Neither the ids nor the table nor lam have to be aligned to more than their elements; node tensors that are not are refused."""
+    def odd(t):
+        room = th.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        room[1:] = t.reshape(-1).to(DEV)
+        return room[1:].view(t.shape)
+
+    for g in (ZOO[2][1], graphs.banded_graph(1, 300, 60)):
+        layer = Layer(g, diff, buckets, 2, 32 if diff else 64, th.bfloat16, seed=22)
+        for plan in (None, layer.plans()[0]):
+            graph, kind = ([plan], "_planned") if plan else ([layer.rows[0], layer.rows[1], layer.rows[3]], "")
+            q, k, v = (t.to(DEV) for t in (layer.q, layer.k, layer.v))
+            call = getattr(graphop, ("attention_diff_forward" if diff else "attention_bucket_forward") + kind)
+            terms = [odd(layer.bucket), odd(layer.table)]
+            more = lambda q: call(*graph, q, k, v, odd(layer.lam), layer.scale, *terms) if diff else call(*graph, q, k, v, *terms, layer.scale)  # noqa: E731
+            assert all(th.equal(a, b) for a, b in zip(more(q)[:2], layer.forward(plan)[:2]))
+            with pytest.raises(RuntimeError, match="not supported"):
+                more(odd(q))
