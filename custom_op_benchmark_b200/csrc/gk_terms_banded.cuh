@@ -66,7 +66,7 @@ struct BandIds {
 };
 // A warp per row (`row` of tile `tile`), four columns per lane at a time.  Bound by its instructions (a select per element) and by the
 // chain node - position - (edge id -) bucket, which every warp goes through once; with one column per lane and step, 443 instructions
-// per row, 4.2M edges took 13 us.
+// per row and the tile's first neighbour found by every block, 4.2M edges took 13 us; so they take 6.7.
 __device__ __forceinline__ void band_ids_row(const BandIds& a, long long tile, int row, const int32_t* __restrict__ bucket, int buckets) {
   const int lane = threadIdx.x & 31, shift = a.per == 32 ? 5 : 4;
   const long long r = tile * kTileM + row;
@@ -208,7 +208,9 @@ struct FwdLayout {
   static constexpr int kCtas = kMaps == 1 ? 3 : 2;
 };
 
-// One block per (tile, head), as attention_forward_kernel.
+// One block per (tile, head), as attention_forward_kernel, and bound like it by the chain load - product - element-wise stage - product
+// behind block-wide barriers: 2 x 8192 nodes, 256 neighbours, 8 heads, a bias 61 us (issue slots 48 %, tensor pipe 11 %, three blocks
+// per SM), two maps 110 us.
 template <int kMaps, bool kBucket>
 __global__ void __launch_bounds__(kThreads, FwdLayout<kMaps>::kCtas)
 terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -735,7 +737,8 @@ __device__ __forceinline__ void terms_backward_tile(const CUtensorMap& map_a, co
 }
 
 // Both sides in one launch, the destination's tiles first: 1024 tiles two to an SM are 3.5 rounds of the chip, which take the time of
-// four; twice as many are seven (2 x 8192 nodes, 8 heads: 78 + 82 us apart).
+// four; twice as many are seven (2 x 8192 nodes, 8 heads: 78 + 82 us apart, 142 together with 24-bit score gradients; two maps without
+// a bias 175).
 template <int kMaps, bool kBucket>
 __global__ void __launch_bounds__(kThreads, 2)
 terms_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -913,7 +916,8 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
 // grid: (blocks, H * maps).  A thread takes 8 elements at a time, so that a warp's loads are whole lines, and asks for kAhead such
 // pieces at once; they go into a table of its own, cell b of thread t at b * NT + t: a warp's 32 cells lie in 32 banks.  An element
 // that takes no part has a gradient of zero and goes to one cell more.  Bound by its instructions, about ten per element (with a test
-// per element and the table's stride not known, 14: 36 us for 6.3M elements of 8 heads), then by reading the gradients.
+// per element and the table's stride not known, 14), then by reading the gradients: 6.3M elements of 8 heads 43 us (3.6 TB/s; 28 when
+// the gradients were bfloat16).
 template <int NT>
 __global__ void __launch_bounds__(NT)
 band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const unsigned short* __restrict__ g, const unsigned char* __restrict__ g_low,
