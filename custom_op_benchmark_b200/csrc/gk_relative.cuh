@@ -11,7 +11,8 @@
 namespace gk {
 
 constexpr int kMostLimits = 1023;
-// A distance fits D: 32 bits between 32-bit positions (limits beyond that are never reached, and left out), else 64.
+// Distances in D: 32 bits between 32-bit positions (limits beyond that are never reached, and left out), and between 64-bit ones where
+// the limits fit, a distance beyond 32 bits standing as the largest that does; else 64.
 // all: with those left out; top: the largest power of two <= n; near: the last limit where that is at most kNear, else -1.
 template <typename D> struct Limits { int n, all, both, top, near; D at[kMostLimits]; };
 
@@ -61,9 +62,12 @@ __device__ __forceinline__ void buckets_of(int (&out)[N], const D (&d)[N], const
 // without a sign: 64-bit positions may lie 2^63 and more apart
 template <typename D, typename P>
 __device__ __forceinline__ D distance(P from, P to, int both, bool& ahead) {
+  using U = std::conditional_t<sizeof(P) == 4, unsigned, unsigned long long>;
   ahead = to > from;
-  const D d = ahead ? (D)to - (D)from : (D)from - (D)to;
-  return ahead && !both ? D(0) : d;
+  const U d = ahead ? (U)to - (U)from : (U)from - (U)to;
+  if (ahead && !both) return D(0);
+  if constexpr (sizeof(D) < sizeof(U)) return d > (U)~D(0) ? ~D(0) : (D)d;
+  else return (D)d;
 }
 
 template <typename P, typename D>
@@ -232,40 +236,51 @@ inline int relative_check(long long C, long long E, const int64_t* limits, int n
   if (n_limits < 0 || (n_limits && !limits)) return GRAPHOP_ERR_INVALID_ARGUMENT;
   return n_limits > kMostLimits ? GRAPHOP_ERR_UNSUPPORTED : GRAPHOP_OK;
 }
-template <typename I> using DistanceOf = std::conditional_t<sizeof(I) == 4, unsigned, unsigned long long>;
+// f(a value of the type of the distances)
+template <typename I, class F>
+inline int with_distance(const int64_t* limits, int n_limits, F&& f) {
+  if constexpr (sizeof(I) == 8)
+    if (n_limits > 0 && limits[n_limits - 1] > 0xffffffffll) return f(0ull);
+  return f(0u);
+}
 
 template <typename I>
 inline int relative_chunks(const I* row, const I* indptr, const I* indices, long long C, long long E, const I* dst_pos, const I* src_pos,
                            const int64_t* limits, int n_limits, int both, int32_t* out, cudaStream_t st) {
-  using D = DistanceOf<I>;
   GK_TRY(relative_check(C, E, limits, n_limits));
-  Limits<D> l;
-  GK_TRY((fill_limits<I, D>(l, limits, n_limits, both)));
-  if (E == 0) return GRAPHOP_OK;
-  if (!row || !indptr || !indices || !out) return GRAPHOP_ERR_INVALID_ARGUMENT;
-  // as many chunks per warp as leave the chip full
-  long long per_warp = C / (148 * 32);
-  per_warp = per_warp < 1 ? 1 : per_warp > 32 ? 32 : per_warp;
-  const long long blocks = (C + 8 * per_warp - 1) / (8 * per_warp);
-  relative_chunks_kernel<I, D><<<(unsigned)(blocks ? blocks : 1), 256, 0, st>>>(row, indptr, C, E, (int)per_warp, indices, dst_pos, src_pos,
-                                                                               l, out);
-  GK_LAUNCHED("relative_buckets");
-  return GRAPHOP_OK;
+  return with_distance<I>(limits, n_limits, [&](auto zero) -> int {
+    using D = decltype(zero);
+    Limits<D> l;
+    GK_TRY((fill_limits<I, D>(l, limits, n_limits, both)));
+    if (E == 0) return GRAPHOP_OK;
+    if (!row || !indptr || !indices || !out) return GRAPHOP_ERR_INVALID_ARGUMENT;
+    // as many chunks per warp as leave the chip full
+    long long per_warp = C / (148 * 32);
+    per_warp = per_warp < 1 ? 1 : per_warp > 32 ? 32 : per_warp;
+    const long long blocks = (C + 8 * per_warp - 1) / (8 * per_warp);
+    relative_chunks_kernel<I, D><<<(unsigned)(blocks ? blocks : 1), 256, 0, st>>>(row, indptr, C, E, (int)per_warp, indices, dst_pos, src_pos,
+                                                                                 l, out);
+    GK_LAUNCHED("relative_buckets");
+    return GRAPHOP_OK;
+  });
 }
 template <typename P>
 inline int relative_planned(const graphop_plan_t* plan, const P* dst_pos, const P* src_pos, const int64_t* limits, int n_limits, int both,
                             int32_t* out, cudaStream_t st) {
-  using D = DistanceOf<P>;
   if (!plan) return GRAPHOP_ERR_INVALID_ARGUMENT;
   GK_TRY(relative_check(plan->n_chunks, plan->n_edges, limits, n_limits));
-  Limits<D> l;
-  GK_TRY((fill_limits<P, D>(l, limits, n_limits, both)));
-  const long long E = plan->n_edges;
-  if (E == 0) return GRAPHOP_OK;
-  if (!plan->erow || !plan->other || !out) return GRAPHOP_ERR_INVALID_ARGUMENT;
-  relative_planned_kernel<P, D><<<(unsigned)((E + kRelTile - 1) / kRelTile), 256, 0, st>>>(plan->erow, plan->other, E, dst_pos, src_pos, l, out);
-  GK_LAUNCHED("relative_buckets");
-  return GRAPHOP_OK;
+  return with_distance<P>(limits, n_limits, [&](auto zero) -> int {
+    using D = decltype(zero);
+    Limits<D> l;
+    GK_TRY((fill_limits<P, D>(l, limits, n_limits, both)));
+    const long long E = plan->n_edges;
+    if (E == 0) return GRAPHOP_OK;
+    if (!plan->erow || !plan->other || !out) return GRAPHOP_ERR_INVALID_ARGUMENT;
+    relative_planned_kernel<P, D><<<(unsigned)((E + kRelTile - 1) / kRelTile), 256, 0, st>>>(plan->erow, plan->other, E, dst_pos, src_pos, l,
+                                                                                            out);
+    GK_LAUNCHED("relative_buckets");
+    return GRAPHOP_OK;
+  });
 }
 
 }  // namespace gk

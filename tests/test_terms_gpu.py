@@ -387,3 +387,19 @@ def test_ids_and_biases_at_odd_addresses(diff, buckets):
             assert all(th.equal(a, b) for a, b in zip(more(q)[:2], layer.forward(plan)[:2]))
             with pytest.raises(RuntimeError, match="not supported"):
                 more(odd(q))
+
+
+@pytest.mark.parametrize("reach", [2 ** 32 - 2 ** 20, 2 ** 40])
+def test_limits_and_distances_around_32_bits(reach):
+    """Limits within 32 bits and beyond, distances from -2^62 to 2^62 with those around every limit and around 2^32."""
+    near = [x + i for x in graphop.bucket_limits(10, reach) + [2 ** 32, 2 ** 31, 2 ** 62] for i in (-1, 0, 1)]
+    at = th.tensor(near + [-x for x in near] + [0])
+    n = len(at)
+    assert (graphop.bucket_limits(10, reach)[-1] >= 2 ** 32) == (reach > 2 ** 32)
+    graph = [th.zeros(1, dtype=th.int64, device=DEV), th.tensor([0, n], device=DEV), th.arange(n, device=DEV)]
+    plan = graphop.GraphPlan(graph[0], graph[1], None, graph[2], 1)
+    zero = th.zeros(1, dtype=th.int64)
+    for both, count in ((False, 10), (True, 20)):
+        want = ref.relative_buckets(th.zeros(n, dtype=th.int64), th.arange(n), count, reach, both, zero, at)
+        assert th.equal(graphop.relative_buckets(*graph, count, reach, both, zero.to(DEV), at.to(DEV)).cpu(), want)
+        assert th.equal(graphop.relative_buckets_planned(plan, count, reach, both, zero.to(DEV), at.to(DEV)).cpu(), want)
