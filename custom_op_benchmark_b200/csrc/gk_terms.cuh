@@ -382,20 +382,26 @@ struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes 
     }
 #pragma unroll
     for (int v = 0; v < N; ++v) {
+      bool part[kMaps];   // by the bias: the row's lse may be NaN
+#pragma unroll
+      for (int m = 0; m < kMaps; ++m) part[m] = active[v];
       if constexpr (kBucket) {
         A b[kMaps];
         Bias::get(b, tab + v * GEO::kHeads * Bias::kBytes);
 #pragma unroll
-        for (int m = 0; m < kMaps; ++m) s[v][m] = b[m] == neg_inf<A>() ? b[m] : s[v][m] + b[m];
+        for (int m = 0; m < kMaps; ++m) {
+          part[m] = part[m] && b[m] != neg_inf<A>();
+          s[v][m] += b[m];
+        }
       }
       A g[kMaps], w = A(0);
 #pragma unroll
       for (int m = 0; m < kMaps; ++m) {
         const A c = m == 0 ? A(1) : -st.lam;
-        const A p = gk_exp2(s[v][m] - st.lse2[m]) * c;
+        const A p = part[m] ? gk_exp2(s[v][m] - st.lse2[m]) * c : A(0);
         w += p;
         g[m] = p * (dp[v] - st.delta[m]);
-        if (!active[v] || (kBucket && p == A(0))) g[m] = A(0);   // a masked row may hold anything
+        if (!part[m] || (kBucket && p == A(0))) g[m] = A(0);   // a masked row may hold anything
       }
       if (active[v] && st.ln.first) {
         EdgePair<A>* at = pd + ((unsigned long long)(pos + v) * (unsigned)Hp + st.ln.head * kMaps);

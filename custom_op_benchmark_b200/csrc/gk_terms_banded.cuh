@@ -626,8 +626,9 @@ __device__ __forceinline__ void terms_backward_tile(const CUtensorMap& map_a, co
 #pragma unroll
               for (int m = 0; m < kMaps; ++m) {
                 const float2 st = kSrc ? s_stat[col * kMaps + m] : make_float2(lse2[m], delta[m]);
-                const float x = score_of<kBucket>(__uint_as_float(raw[m][j + e]), sl2, s_table + m * 256, ident, col >= jlo && col <= jhi);
-                const float pr = exp2_fast(x - st.x) * (m == 0 ? 1.f : -lam);
+                const float b = kBucket ? s_table[m * 256 + ident] : 0.f;
+                const bool part = kBucket ? b != -INFINITY : col >= jlo && col <= jhi;   // not by the score: st.x may be NaN
+                const float pr = part ? exp2_fast(fmaf(__uint_as_float(raw[m][j + e]), sl2, b) - st.x) * (m == 0 ? 1.f : -lam) : 0.f;
                 w[e] += pr;
                 const float gr = pr * (__uint_as_float(raw[kMaps][j + e]) - st.y);
                 g[m][e] = pr == 0.f ? 0.f : gr;   // dP of a position that takes no part may be anything
@@ -880,7 +881,7 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
             if (pr != 0.f) { acc[m][0] = fmaf(pr, u.x, acc[m][0]); acc[m][1] = fmaf(pr, u.y, acc[m][1]); }
           } else {
             const float2 st = t.stat[((kSide == 2 ? c : r) * t.H + head) * kMaps + m];
-            const float pr = exp2_fast(sm - st.x) * (m == 0 ? 1.f : -lam);
+            const float pr = bias[m] == -INFINITY ? 0.f : exp2_fast(sm - st.x) * (m == 0 ? 1.f : -lam);
             const float g = pr == 0.f ? 0.f : pr * (dp - st.y);
             w += pr;
             if (m == mine) own = g;

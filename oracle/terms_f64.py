@@ -60,7 +60,7 @@ def attention(dst, src, q, k, v, scale, bucket=None, table=None, lam=None, d_o=N
     top0 = th.where(top == -float("inf"), th.zeros_like(top), top)
     w = th.where(part, th.exp(s - top0[dst]), th.zeros_like(s))
     total = th.zeros(n, maps, dtype=F64, device=dev).index_add(0, dst, w)
-    p = w / th.where(total == 0, th.ones_like(total), total)[dst]
+    p = th.where(part, w / th.where(total == 0, th.ones_like(total), total)[dst], th.zeros_like(w))   # the total may be NaN
     r = dict(dst=dst, src=src, part=part, bias=bias, p=p, qe=qe, ke=ke, lse=th.where(total == 0, top, top0 + total.log()))
     ve = _rows(v, src, part)
     per = ve if not diff else ve.repeat_interleave(2, 1)           # the row of v that a map's probability multiplies
@@ -78,7 +78,7 @@ def attention(dst, src, q, k, v, scale, bucket=None, table=None, lam=None, d_o=N
     dp = (gper * per).sum(-1)
     d_full = th.nan_to_num(d_o.to(F64)) if not diff else th.nan_to_num(d_o.to(F64)).repeat_interleave(2, 1)
     delta = (d_full * sums).sum(-1)
-    g = sign * p * (dp - delta[dst])
+    g = th.where(part, sign * p * (dp - delta[dst]), th.zeros_like(p))
     wt = sign * p
     wt = wt if not diff else wt[:, 0::2] + wt[:, 1::2]
     r.update(ge=ge, gper=gper, dp=dp, delta=delta, g=g, d_full=d_full)
