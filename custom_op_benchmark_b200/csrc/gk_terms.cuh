@@ -497,7 +497,8 @@ struct TermsBwdDst : GEO, Shape<GEO, 2, kBucket ? TermsBias<GEO, kMaps>::kBytes 
 };
 
 // Source side: the plain layer's sums over the transposed CSR with pairs (w, g), a head per map.  The scale is applied once per
-// row, so that dT has the unscaled g; pairs of zeros are passed over, so that a masked position's rows of q and dO may hold anything.
+// row, so that dT has the unscaled g; a weight or score gradient of zero is passed over, so that what takes no part, a position or one
+// map of it, may have anything in its rows of q and dO.
 template <class GEO>
 struct TermsBwdSrc : GroupAttnBwdSrc<GEO, true> {
   using Base = GroupAttnBwdSrc<GEO, true>;
@@ -516,9 +517,13 @@ struct TermsBwdSrc : GroupAttnBwdSrc<GEO, true> {
       this->load_staged(fg, slot + v * this->kStepBytes + kRow);
       A w, g;
       lds2(w, g, tab + v * GEO::kHeads * 2 * (int)sizeof(A));
-      if (w != A(0) || g != A(0)) {
+      if (w != A(0)) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) { st.av[i].axpy(w, fg[i]); st.ak[i].axpy(g, fq[i]); }
+        for (int i = 0; i < W; ++i) st.av[i].axpy(w, fg[i]);
+      }
+      if (g != A(0)) {   // zero alone where the other map takes part
+#pragma unroll
+        for (int i = 0; i < W; ++i) st.ak[i].axpy(g, fq[i]);
       }
     }
   }
@@ -546,10 +551,8 @@ struct TermsSumPairs : SumAttnPairs<GEO> {
     frag_unpack<T, GEO::SB>(fg, r.g);
     A w, g;
     lds2(w, g, tab);
-    if (w != A(0) || g != A(0)) {
-      st.av[0].axpy(w, fg);
-      st.ak[0].axpy(g, fq);
-    }
+    if (w != A(0)) st.av[0].axpy(w, fg);
+    if (g != A(0)) st.ak[0].axpy(g, fq);
   }
   __device__ __forceinline__ void store_row(State& st, int node) const {
     this->flush(st);

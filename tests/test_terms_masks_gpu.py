@@ -83,3 +83,29 @@ def test_tensor_cores(diff, buckets, how):
     plans = layer.plans()
     assert plans[0].dense_band and plans[1].dense_band
     _check(layer, *spoilt[:2], layer.step(plans), how, 300, *spoilt[2:])
+
+@pytest.mark.parametrize("dt", [th.float32, th.bfloat16], ids=str)
+@pytest.mark.parametrize("planned", [False, True])
+def test_one_map_masked_where_the_other_is_not(dt, planned):
+    """Map 0 of node 77 is spoilt by two live edges; its other edges take part in map 1 alone, and nothing of them changes."""
+    g = graphs.banded_graph(1, 200, 20)
+    layer = Layer(g, True, 7, 2, 32, dt, seed=33)
+    dst, src = ref.dst_of_edges(g.indptr), g.indices.long()
+    layer.table[5, 0] = -math.inf
+    layer.bucket[layer.bucket == 5] = 4
+    layer.bucket[layer.bucket == 1] = 0
+    mine = (dst == 77).nonzero().flatten()
+    layer.bucket[mine] = 5                      # map 0 of head 0 sees nothing of these
+    layer.bucket[mine[:2]] = 1
+    r = layer.reference()
+    staged = STAGED if planned and dt == th.bfloat16 else 0.0
+    b = ref.bounds(r, layer.q, layer.k, layer.v, layer.scale, layer.dt, layer.bucket, layer.table, staged)
+    layer.q[77, 0] = math.nan
+    got = dict(zip(layer.names(), layer.step(layer.plans() if planned else None)))
+    assert bool(th.isnan(got["o"][77, 0]).all()) and bool((got["d_table"][5, 0] == 0).all())
+    keep = {name: th.ones(len(r[name]), dtype=th.bool) for name in ("o", "dq", "dk", "dv", "d_table")}
+    keep["o"][77] = keep["dq"][77] = False
+    keep["dk"][src[mine[:2]]] = keep["dv"][src[mine[:2]]] = False
+    keep["d_table"][1] = False
+    for name, rows in keep.items():
+        ref.assert_within(got[name].detach().cpu()[rows], r[name][rows], b[name][rows], name)
