@@ -725,16 +725,24 @@ inline int banded_terms_backward(const graphop_plan_t*, const graphop_plan_t*, c
   return GRAPHOP_ERR_UNSUPPORTED;
 }
 
-// The geometry of a row: the plain layer's, but blocks of as many heads as divide their number, where that makes every lane own whole
-// slots known at compile time.
-template <typename T>
-inline GeoPick terms_geo(int H, int D) {
-  const GeoPick p = pick_geo(H, D, sizeof(T), 16, false);
+// The geometry of a row of H heads of D elements of `elem` bytes: the plain layer's, but blocks of as many heads as divide their number,
+// where that makes every lane own whole slots known at compile time.
+inline GeoPick terms_geo(int H, int D, int elem) {
+  const GeoPick p = pick_geo(H, D, elem, 16, false);
   if (p.LT || (H & (H - 1)) == 0) return p;
-  GeoPick q = pick_geo(H & -H, D, sizeof(T), 16, false);   // the largest power of two in H
+  GeoPick q = pick_geo(H & -H, D, elem, 16, false);   // the largest power of two in H
   if (!q.LT) return p;
   q.nhb = H / (q.G / q.L);
   return q;
+}
+// Carry levels of the walks of such rows, in whatever geometry of the two walkers they get.  Blocks that divide the number of heads may be
+// many more than walk_bytes counts, each with records and their ids (8-byte elements, 47 heads of 8: 47 blocks of 4 lanes for 6 of 16 x 2
+// slots; 6016 bytes of sums and 188 of ids for 6144 and 24).
+inline size_t terms_walk_bytes(long long E, long long n_nodes, int H, int D, int elem, int accs, int stats) {
+  const GeoPick p = terms_geo(H, D, elem);
+  const size_t most = walk_bytes(E, n_nodes, H, D, elem, false, accs, stats);
+  const size_t own = carry_bytes(tile_bound(E, n_nodes), p.nhb, (long long)accs * p.accs(elem) + stats * p.G, elem == 8 ? 8 : 4);
+  return p.SB && own > most ? own : most;
 }
 
 template <typename T>
@@ -745,7 +753,7 @@ inline int terms_check(const TermsCall<T>& c, long long C, bool al, GeoPick* geo
   if (c.buckets > kMostBuckets) return GRAPHOP_ERR_UNSUPPORTED;
   if (!is_pow2(c.D * (int)sizeof(T) / 16) || c.D * (int)sizeof(T) % 16) return GRAPHOP_ERR_UNSUPPORTED;
   if (!attention_shape_ok<T>(c.H, c.row_d(), al, geo)) return GRAPHOP_ERR_UNSUPPORTED;
-  *geo = terms_geo<T>(c.H, c.row_d());
+  *geo = terms_geo(c.H, c.row_d(), sizeof(T));
   return GRAPHOP_OK;
 }
 inline bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -813,7 +821,7 @@ inline int run_terms_src(Arena& ar, const GraphView& g, const TermsCall<T>& c, c
                          T* dv, cudaStream_t st) {
   const int H = c.H * c.maps(), D = c.D;
   const long long table = (long long)c.node_bytes(c.n_dst);
-  const GeoPick s = terms_geo<T>(H, D);
+  const GeoPick s = terms_geo(H, D, sizeof(T));
   const auto ring = [&](int only, int most) -> int {
     return dispatch_geo<T, false, true>(s, [&](auto tag) -> int {
       TermsBwdSrc<typename decltype(tag)::type> op;
@@ -897,11 +905,11 @@ inline size_t terms_bytes(bool diff, bool backward, long long E, long long n_nod
   const size_t acc = elem == 8 ? 8 : 4;
   const int maps = diff ? 2 : 1, columns = H * maps, row_d = D * maps;
   size_t need = graph_bytes(E, n_nodes, index_bytes);
-  if (!backward) return need + walk_bytes(E, n_nodes, H, row_d, elem, false, maps, 2 * maps) + kAlign;
+  if (!backward) return need + terms_walk_bytes(E, n_nodes, H, row_d, elem, maps, 2 * maps) + kAlign;
   need += align_up((size_t)E * stat_heads(columns, (int)acc) * 2 * acc);
   if (diff) need += align_up((size_t)n_nodes * H * acc) + bucket_sum_bytes(n_nodes, H, 1, (int)acc);
   if (buckets) need += bucket_sum_bytes(E, columns, buckets, (int)acc);
-  const size_t dst = walk_bytes(E, n_nodes, H, row_d, elem, false, 1, 0), src = walk_bytes(E, n_nodes, columns, D, elem, false, 2, 0);
+  const size_t dst = terms_walk_bytes(E, n_nodes, H, row_d, elem, 1, 0), src = terms_walk_bytes(E, n_nodes, columns, D, elem, 2, 0);
   return need + (dst > src ? dst : src) + kAlign;
 }
 

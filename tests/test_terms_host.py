@@ -1,10 +1,13 @@
 """Attention layers with learned score terms, more of what needs no GPU."""
 import math
+import os
+import subprocess
 
 import pytest
 import torch as th
 
-from helpers import random_graph
+from helpers import ROOT, random_graph
+from custom_op_benchmark_b200 import build
 from oracle import terms_f64 as ref
 
 
@@ -28,3 +31,13 @@ def test_reference_leaves_masked_edges_out_of_a_spoilt_row(diff):
         assert th.equal(th.isnan(r[name]), th.isnan(few[name])), name
         assert th.equal(th.nan_to_num(r[name]), th.nan_to_num(few[name])), name
     assert bool(th.isnan(r["dq"][5]).any()) and not bool(th.isnan(r["d_table"][4]).any())
+
+
+def test_every_shape_fits_the_workspace_it_asks_for(tmp_path):
+    """A program that takes a call's buffers as the library does, over all head counts and widths of all types, without a device."""
+    exe = tmp_path / "terms_workspace"
+    res = subprocess.run([build._nvcc(), "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a", "-I" + build.CSRC,
+                          os.path.join(ROOT, "tests", "terms_workspace.cu"), "-o", str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    res = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stdout
