@@ -210,18 +210,30 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// (n, H, 64) bf16 node tensor as a 3-D map (feature, head, node), boxes of 64 nodes of one head, 128-byte swizzle
-inline bool make_map(CUtensorMap* map, const void* base, long long n, int H) {
+// (n, H, 64) bf16 node tensor as a 3-D map (feature, head, node), boxes of `rows` nodes of one head, 128-byte swizzle.  The driver wants a
+// current context, which a host thread has from its first call of the runtime that needs one on: autograd's thread comes here
+// before that, in the first backward pass of a process.
+inline bool make_map_rows(CUtensorMap* map, const void* base, long long n, int H, int rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)H, (cuuint64_t)n};
   const cuuint64_t strides[2] = {(cuuint64_t)kRowBytes, (cuuint64_t)H * kRowBytes};
-  const cuuint32_t box[3] = {(cuuint32_t)kD, 1u, (cuuint32_t)kKeys};
+  const cuuint32_t box[3] = {(cuuint32_t)kD, 1u, (cuuint32_t)rows};
   const cuuint32_t estr[3] = {1u, 1u, 1u};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const auto encode = [&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = encode();
+  if (rc == CUDA_ERROR_INVALID_CONTEXT || rc == CUDA_ERROR_NOT_INITIALIZED) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+    rc = encode();
+  }
+  return rc == CUDA_SUCCESS;
 }
+inline bool make_map(CUtensorMap* map, const void* base, long long n, int H) { return make_map_rows(map, base, n, H, kKeys); }
 
 }  // namespace banded
 }  // namespace gk

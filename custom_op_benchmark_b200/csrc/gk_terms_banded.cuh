@@ -1001,19 +1001,6 @@ inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, 
   return GRAPHOP_OK;
 }
 
-// (n, H, 64) bf16 node tensor as make_map's, in boxes of `rows` nodes
-inline bool make_map_rows(CUtensorMap* map, const void* base, long long n, int H, int rows) {
-  auto fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)H, (cuuint64_t)n};
-  const cuuint64_t strides[2] = {(cuuint64_t)kRowBytes, (cuuint64_t)H * kRowBytes};
-  const cuuint32_t box[3] = {(cuuint32_t)kD, 1u, (cuuint32_t)rows};
-  const cuuint32_t estr[3] = {1u, 1u, 1u};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 inline int band_pitch(const graphop_plan_t* plan) { return (plan->band_span + kKeys - 1) / kKeys * kKeys; }
 inline long long band_tiles_of(long long n) { return (n + kTileM - 1) / kTileM; }
 inline bool band_plan_ok(const graphop_plan_t* plan, long long n, int H) {
