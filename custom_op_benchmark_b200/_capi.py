@@ -111,6 +111,7 @@ TERMS_PLANNED_SIGNATURES = {
 }
 TERMS_UNTYPED = {
     "graphop_terms_workspace_bytes": ([_INT, _I64, _I64] + [_INT] * 5, _SZ),
+    "graphop_terms_workspace_bytes_planned": ([_INT, _PP, _PP, _I64, _I64] + [_INT] * 4, _SZ),
     "graphop_relative_buckets_i32": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64, _P], _INT),
     "graphop_relative_buckets_i64": ([_P] * 3 + [_I64] + [_P] * 3 + [_INT] * 2 + [_P, _I64, _P], _INT),
     "graphop_relative_buckets_planned_i32": ([_PP] + [_P] * 3 + [_INT] * 2 + [_P] * 2, _INT),

@@ -661,8 +661,12 @@ void check_terms_plan(const PlanHandle& plan_r, int64_t n) {
   if (n < plan_r.graph->plan.n_nodes)
     fail("q must have a row for each of the plan's " + std::to_string(plan_r.graph->plan.n_nodes) + " nodes");
 }
-void terms_workspace(Call& c, int op, int64_t e, const TermsShape& s, const Tensor& like, int index_bytes) {
-  c.bytes = graphop_terms_workspace_bytes(op, e, std::max(s.n, s.m), s.H, s.D, s.buckets, (int)like.element_size(), index_bytes);
+// rows: the plan of a call on plans, else null; cols: of its backward alone
+void terms_workspace(Call& c, int op, int64_t e, const TermsShape& s, const Tensor& like, int index_bytes, const GraphPtr& rows,
+                     const GraphPtr& cols) {
+  const int elem = (int)like.element_size();
+  c.bytes = rows ? graphop_terms_workspace_bytes_planned(op, &rows->plan, cols ? &cols->plan : nullptr, s.n, s.m, s.H, s.D, s.buckets, elem)
+                 : graphop_terms_workspace_bytes(op, e, std::max(s.n, s.m), s.H, s.D, s.buckets, elem, index_bytes);
   c.scratch = at::empty({(int64_t)c.bytes + 256}, like.options().dtype(at::kByte));
   c.ws = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(c.scratch.data_ptr()) + 255) / 256 * 256);
 }
@@ -699,7 +703,7 @@ struct TermsBackward : GraphNode {
     Tensor dq = at::empty_like(x.q.detach()), dk = at::empty_like(x.k.detach()), dv = at::empty_like(x.v.detach()), dl, dt;
     if (diff) dl = at::empty_like(x.lam.detach());
     if (s.buckets) dt = at::empty_like(x.table.detach());
-    terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_BWD : GRAPHOP_TERMS_BUCKET_BWD, e, s, x.q, ib);
+    terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_BWD : GRAPHOP_TERMS_BUCKET_BWD, e, s, x.q, ib, rows, cols);
     const char* what = diff ? "attention_diff_backward" : "attention_bucket_backward";
     // f(graph arguments..., then) with `then` the arguments after the graph's
     const auto typed = [&](auto* y, auto&& call) {
@@ -765,7 +769,7 @@ TermsOutputs terms_forward(const TermsGraph& graph, const TermsInputs& x, bool d
   const auto acc = s.elem == 1 ? at::kDouble : at::kFloat;
   if (diff && (grads || keep)) parts = at::empty({s.n, s.H, 2, 2 * s.D}, x.q.options().dtype(acc));
   if (!diff && (grads || keep) && x.q.scalar_type() != acc) parts = at::empty(o.sizes(), x.q.options().dtype(acc));   // else o serves
-  terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_FWD : GRAPHOP_TERMS_BUCKET_FWD, e, s, x.q, ib);
+  terms_workspace(c, diff ? GRAPHOP_TERMS_DIFF_FWD : GRAPHOP_TERMS_BUCKET_FWD, e, s, x.q, ib, graph.rows, nullptr);
   const auto typed = [&](auto* y, auto&& call) {
     using E = std::remove_pointer_t<decltype(y)>;
     const E *q = ptr<E>(x.q), *k = ptr<E>(x.k), *v = ptr<E>(x.v), *lam = ptr<E>(x.lam), *table = ptr<E>(x.table);

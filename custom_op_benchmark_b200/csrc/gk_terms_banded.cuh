@@ -17,14 +17,12 @@
 // A product takes whole blocks: 0 * NaN from a row that takes no part, or that lies next to the band, reaches every row of the
 // tile.  A tile that ends with a value that is not finite says so in `dirty`, and band_again_kernel does it again edge by edge.
 #pragma once
-#include "gk_band_tiles.cuh"
-#include "gk_terms.cuh"
+#include "gk_terms_band.cuh"
 
 namespace gk {
 namespace banded {
 
 constexpr unsigned kNoPart = 255;                 // id of an element that takes no part
-constexpr int kMostBandBuckets = 255;
 
 struct TermsTile {
   const __nv_bfloat16 *table, *lam;          // (buckets, H * maps), (H)
@@ -969,20 +967,6 @@ band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const unsigned sho
     if (lane == 0) partial[((size_t)blockIdx.x * buckets + b) * columns + column] = s;
   }
 }
-// A block has a table per thread; as many blocks as share the SMs' memory, a piece or more for every thread.
-struct BandSumShape { int threads, smem, blocks; };
-inline BandSumShape band_sum_shape(long long elements, int buckets, int columns) {
-  BandSumShape s;
-  s.threads = 128;
-  while (s.threads > 32 && (buckets + 1) * s.threads * (int)sizeof(float) > 56 * 1024) s.threads >>= 1;
-  s.smem = (buckets + 1) * s.threads * (int)sizeof(float);
-  long long per_sm = 200 * 1024 / (s.smem + 1024);
-  per_sm = per_sm > 10 ? 10 : per_sm;
-  long long blocks = per_sm * 148 / columns, most = elements / 8 / s.threads + 1;
-  blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
-  s.blocks = (int)blocks;
-  return s;
-}
 inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, const unsigned short* g, const unsigned char* g_low,
                                long long elements, int buckets, int columns, double* partial, __nv_bfloat16* out, cudaStream_t st) {
   const auto launch = [&](auto kernel, std::atomic<bool> (&configured)[64]) -> int {
@@ -1001,12 +985,6 @@ inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, 
   return GRAPHOP_OK;
 }
 
-inline int band_pitch(const graphop_plan_t* plan) { return (plan->band_span + kKeys - 1) / kKeys * kKeys; }
-inline long long band_tiles_of(long long n) { return (n + kTileM - 1) / kTileM; }
-inline bool band_plan_ok(const graphop_plan_t* plan, long long n, int H) {
-  return (plan->flags & GRAPHOP_PLAN_DENSE_BAND) && plan->band_span > 0 && plan->band_span <= kSpan && plan->node_lo && plan->node_deg &&
-         plan->node_first && plan->tile_lo && n >= 1 && n <= plan->n_nodes && H <= 65535;
-}
 inline BandIds band_ids_of(const graphop_plan_t* plan, const int32_t* eid, long long n, int per, unsigned char* ids) {
   return BandIds{plan->node_lo, plan->node_deg, plan->node_first, plan->tile_lo, eid, n, band_pitch(plan), per, ids};
 }
@@ -1024,9 +1002,10 @@ inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat
   using L = FwdLayout<kMaps>;
   const int pitch = band_pitch(plan);
   const long long tiles = band_tiles_of(c.n_dst);
+  const BandRoom room = band_room_forward(ar, plan, c.n_dst, c.H, c.buckets);
   TermsTile t{};
-  t.ids = kBucket ? (unsigned char*)ar.take((size_t)tiles * pitch * kTileM) : nullptr;
-  t.dirty = (int*)ar.take((size_t)tiles * c.H * sizeof(int));
+  t.ids = room.ids;
+  t.dirty = room.dirty;
   if (ar.overflow) return GRAPHOP_ERR_UNSUPPORTED;
   CUtensorMap mq, mk, mv;
   if (!make_map(&mq, c.q, c.n_dst, c.H) || !make_map(&mk, c.k, c.n_src, c.H) || !make_map(&mv, c.v, c.n_src, c.H))
@@ -1035,7 +1014,7 @@ inline int terms_forward(const graphop_plan_t* plan, const TermsCall<__nv_bfloat
   GK_TRY(allow_smem(terms_forward_kernel<kMaps, kBucket>, L::kBytes, configured));
   if (kBucket) {
     band_ids_kernel<<<dim3((unsigned)tiles, kTileM / 8), 256, 0, st>>>(
-        band_ids_of(plan, nullptr, c.n_dst, 32, const_cast<unsigned char*>(t.ids)), c.bucket, c.buckets);
+        band_ids_of(plan, nullptr, c.n_dst, 32, room.ids), c.bucket, c.buckets);
     GK_LAUNCHED("band_ids");
   }
   t.table = c.table; t.lam = c.lam; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan->node_lo; t.node_deg = plan->node_deg;
@@ -1053,27 +1032,11 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   using LD = BwdLayout<false, kMaps>;
   using LS = BwdLayout<true, kMaps>;
   const int pitch = band_pitch(plan_r), pitch_t = band_pitch(plan_t), columns = c.H * kMaps;
-  const long long tiles = band_tiles_of(c.n_dst), tiles_t = band_tiles_of(c.n_src), elements = tiles * pitch * kTileM;
-  const BandSumShape sum = kBucket ? band_sum_shape(elements, c.buckets, columns) : BandSumShape{};
-
+  const long long tiles = band_tiles_of(c.n_dst), tiles_t = band_tiles_of(c.n_src);
+  const BandRoom room = band_room_backward(ar, plan_r, plan_t, c.n_dst, c.n_src, c.H, kMaps, c.buckets);
+  if (room.bytes > ar.cap) return GRAPHOP_ERR_UNSUPPORTED;
   TermsTile t{};
-  t.stat = (float2*)ar.take((size_t)c.n_dst * columns * sizeof(float2));
-  t.dirty = (int*)ar.take((size_t)tiles * c.H * sizeof(int));
-  int* dirty_t = (int*)ar.take((size_t)tiles_t * c.H * sizeof(int));
-  unsigned char *ids = nullptr, *ids_t = nullptr;
-  double* partial = nullptr;
-  float* t2 = kMaps == 2 ? (float*)ar.take((size_t)c.n_dst * c.H * sizeof(float)) : nullptr;
-  if (kBucket) {
-    ids = (unsigned char*)ar.take((size_t)elements);
-    ids_t = (unsigned char*)ar.take((size_t)tiles_t * pitch_t * kTileM);
-    t.g = (unsigned short*)ar.take((size_t)columns * elements * 2);
-    t.g_low = (unsigned char*)ar.take((size_t)columns * elements);
-    partial = (double*)ar.take((size_t)sum.blocks * c.buckets * columns * sizeof(double));
-  }
-  const size_t before_sum = ar.used;
-  if (kMaps == 2) ar.take(bucket_sum_bytes(c.n_dst, c.H, 1, 4));
-  if (ar.overflow) return GRAPHOP_ERR_UNSUPPORTED;
-  ar.used = before_sum;
+  t.stat = room.stat; t.dirty = room.dirty; t.g = room.g; t.g_low = room.g_low;
   CUtensorMap mq, mk, mv, mg, mqs, mgs;
   if (!make_map(&mq, c.q, c.n_dst, c.H) || !make_map(&mk, c.k, c.n_src, c.H) || !make_map(&mv, c.v, c.n_src, c.H) ||
       !make_map(&mg, dout, c.n_dst, c.H) || !make_map_rows(&mqs, c.q, c.n_dst, c.H, LS::kB) ||
@@ -1082,35 +1045,33 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   constexpr int smem = LD::kBytes > LS::kBytes ? LD::kBytes : LS::kBytes;
   static std::atomic<bool> configured[64];
   GK_TRY(allow_smem(terms_backward_kernel<kMaps, kBucket>, smem, configured));
-  const BandIds own = band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, ids), other = band_ids_of(plan_t, plan_t->eid, c.n_src, LS::kC, ids_t);
+  const BandIds own = band_ids_of(plan_r, nullptr, c.n_dst, LD::kC, room.ids), other = band_ids_of(plan_t, plan_t->eid, c.n_src, LS::kC, room.ids_t);
   band_prepare_kernel<kMaps, kBucket><<<dim3((unsigned)(kBucket && tiles_t > tiles ? tiles_t : tiles), kTileM / 8, kBucket ? 3 : 1), 256, 0, st>>>(
-      own, other, c.bucket, c.buckets, (const float*)sums, dout, (const float*)lse, c.n_dst * c.H, t.stat, t2);
+      own, other, c.bucket, c.buckets, (const float*)sums, dout, (const float*)lse, c.n_dst * c.H, t.stat, room.t2);
   GK_LAUNCHED("band_prepare");
-  t.table = c.table; t.lam = c.lam; t.ids = ids; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan_r->node_lo;
+  t.table = c.table; t.lam = c.lam; t.ids = room.ids; t.pitch = pitch; t.buckets = c.buckets; t.node_lo = plan_r->node_lo;
   t.node_deg = plan_r->node_deg; t.n_own = c.n_dst; t.n_other = c.n_src; t.H = c.H; t.scale = (float)c.scale; t.out0 = dq;
   TermsTile u = t;
-  u.ids = ids_t; u.pitch = pitch_t; u.node_lo = plan_t->node_lo; u.node_deg = plan_t->node_deg; u.dirty = dirty_t; u.n_own = c.n_src;
+  u.ids = room.ids_t; u.pitch = pitch_t; u.node_lo = plan_t->node_lo; u.node_deg = plan_t->node_deg; u.dirty = room.dirty_t; u.n_own = c.n_src;
   u.n_other = c.n_dst; u.out0 = dk; u.out1 = dv;
   terms_backward_kernel<kMaps, kBucket><<<dim3((unsigned)(tiles > tiles_t ? tiles : tiles_t), (unsigned)c.H, 2), kThreads, smem, st>>>(
       mq, mk, mv, mg, mqs, mgs, t, u, (unsigned)tiles, (unsigned)tiles_t);
   GK_LAUNCHED(kMaps == 2 ? "attention_diff_bwd_banded" : "attention_bucket_bwd_banded");
   GK_TRY((run_band_again<1, kMaps, kBucket>(AgainArgs{t, c.q, c.k, c.v, dout, plan_r->node_first, nullptr, c.bucket, (int)tiles}, st)));
   GK_TRY((run_band_again<2, kMaps, kBucket>(AgainArgs{u, c.q, c.k, c.v, dout, plan_t->node_first, plan_t->eid, c.bucket, (int)tiles_t}, st)));
-  if (kBucket) GK_TRY(run_band_bucket_sum(sum, ids, t.g, t.g_low, elements, c.buckets, columns, partial, d_table, st));
-  if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));
+  if (kBucket) GK_TRY(run_band_bucket_sum(room.sum, room.ids, room.g, room.g_low, room.elements, c.buckets, columns, room.partial, d_table, st));
+  if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, room.t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));
   return GRAPHOP_OK;
 }
 
 }  // namespace banded
 
-// Heads of 64 features of v in bfloat16 on a dense band, up to 255 buckets, where the caller's workspace holds the tiles' ids and
-// score gradients: sized for the walkers' pairs and records it does but for very large batches of narrow bands.
-// GRAPHOP_ERR_UNSUPPORTED else: the caller then runs the walkers.
+// Where band_serves and the workspace is as large as graphop_terms_workspace_bytes_planned asks; GRAPHOP_ERR_UNSUPPORTED else: the caller
+// then runs the walkers.
 template <>
 inline int banded_terms_forward<__nv_bfloat16>(const graphop_plan_t* plan, const TermsCall<__nv_bfloat16>& c, __nv_bfloat16* o,
                                                void* sums, void* lse, void* ws, size_t wsb, cudaStream_t st) {
-  if (c.row_d() != banded::kD || c.buckets > banded::kMostBandBuckets || c.n_src < 1 || !banded::band_plan_ok(plan, c.n_dst, c.H) ||
-      ((uintptr_t)sums & 31))   // store_sums16's alignment
+  if (!banded::band_serves(plan, nullptr, c.n_dst, c.n_src, c.H, c.row_d(), c.buckets) || ((uintptr_t)sums & 31))   // store_sums16's alignment
     return GRAPHOP_ERR_UNSUPPORTED;
   Arena ar(ws, wsb);
   if (!c.diff) return banded::terms_forward<1, true>(plan, c, o, sums, lse, ar, st);
@@ -1122,9 +1083,7 @@ inline int banded_terms_backward<__nv_bfloat16>(const graphop_plan_t* plan_r, co
                                                 const TermsCall<__nv_bfloat16>& c, const void* sums, const void* lse,
                                                 const __nv_bfloat16* dout, __nv_bfloat16* dq, __nv_bfloat16* dk, __nv_bfloat16* dv,
                                                 __nv_bfloat16* d_table, __nv_bfloat16* d_lam, void* ws, size_t wsb, cudaStream_t st) {
-  if (c.row_d() != banded::kD || c.buckets > banded::kMostBandBuckets || !banded::band_plan_ok(plan_r, c.n_dst, c.H) ||
-      !banded::band_plan_ok(plan_t, c.n_src, c.H))
-    return GRAPHOP_ERR_UNSUPPORTED;
+  if (!banded::band_serves(plan_r, plan_t, c.n_dst, c.n_src, c.H, c.row_d(), c.buckets)) return GRAPHOP_ERR_UNSUPPORTED;
   Arena ar(ws, wsb);
   if (!c.diff) return banded::terms_backward<1, true>(plan_r, plan_t, c, sums, lse, dout, dq, dk, dv, d_table, d_lam, ar, st);
   if (c.buckets) return banded::terms_backward<2, true>(plan_r, plan_t, c, sums, lse, dout, dq, dk, dv, d_table, d_lam, ar, st);

@@ -841,12 +841,15 @@ def _same_device(first, *others):
             raise RuntimeError("expected all tensors of the call on %s" % first.device)
 
 
-def _terms_call(name, graph, elem, op_id, n_edges, n_nodes, h, d, buckets, device, args):
-    """One call of include/graphop_terms.h.  graph: (index suffix, bytes, arguments) of a chunk table, or plans."""
+def _terms_call(name, graph, elem, op_id, n_edges, nodes, h, d, buckets, device, args):
+    """One call of include/graphop_terms.h.  graph: (index suffix, bytes, arguments) of a chunk table, or plans; nodes: (n_dst, n_src)."""
     lib = _capi.lib()
     planned = graph[0] is None
     with th.cuda.device(device):
-        need = lib.graphop_terms_workspace_bytes(op_id, n_edges, n_nodes, h, d, buckets, elem[1], graph[1])
+        if planned:
+            need = lib.graphop_terms_workspace_bytes_planned(op_id, *(graph[2] + [None])[:2], *nodes, h, d, buckets, elem[1])
+        else:
+            need = lib.graphop_terms_workspace_bytes(op_id, n_edges, max(nodes), h, d, buckets, elem[1], graph[1])
         _ws, base, need = _scratch(need, device)
         fn = getattr(lib, "graphop_%s_planned_%s" % (name, elem[0]) if planned else "graphop_%s_%s_%s" % (name, elem[0], graph[0]))
         _check(fn(*graph[2], *args, base, need, th.cuda.current_stream(device).cuda_stream), name + ("_planned" if planned else ""))
@@ -904,7 +907,7 @@ def _bucket_forward(graph, e, q, k, v, bucket, table, scale, keep_sums):
     o = th.empty_like(q)
     sums = th.empty_like(q, dtype=_lse_dtype(q)) if keep_sums and q.dtype != _lse_dtype(q) else None
     lse = th.empty((q.size(0), h), dtype=_lse_dtype(q), device=q.device)
-    _terms_call("attention_bucket_forward", graph, elem, _capi.TERMS_BUCKET_FWD, e, max(q.size(0), k.size(0)), h, d, nb, q.device,
+    _terms_call("attention_bucket_forward", graph, elem, _capi.TERMS_BUCKET_FWD, e, (q.size(0), k.size(0)), h, d, nb, q.device,
                 [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, float(scale), _p(o), _p(sums), _p(lse)] + ([] if graph[0] is None else [e])
                 + [q.size(0), k.size(0), h, d])
     return (o, lse, o if sums is None else sums) if keep_sums else (o, lse)
@@ -921,7 +924,7 @@ def _bucket_backward(graph, e, q, k, v, bucket, table, sums, lse, d_o, scale):
             or lse.dtype != _lse_dtype(q):
         raise RuntimeError("sums, lse and d_o must have the forward's shapes and types")
     out = [th.empty_like(t) for t in (q, k, v, table)]
-    _terms_call("attention_bucket_backward", graph, elem, _capi.TERMS_BUCKET_BWD, e, max(q.size(0), k.size(0)), h, d, nb, q.device,
+    _terms_call("attention_bucket_backward", graph, elem, _capi.TERMS_BUCKET_BWD, e, (q.size(0), k.size(0)), h, d, nb, q.device,
                 [_p(q), _p(k), _p(v), _p(bucket), _p(table), nb, _p(sums), _p(lse), _p(d_o), float(scale)] + [_p(t) for t in out]
                 + ([] if graph[0] is None else [e]) + [q.size(0), k.size(0), h, d])
     return out
@@ -978,7 +981,7 @@ def _diff_forward(graph, e, q, k, v, lam, scale, bucket, table, keep_parts):
     o = th.empty((n, h, 2 * d), dtype=q.dtype, device=q.device)
     parts = th.empty((n, h, 2, 2 * d), dtype=_lse_dtype(q), device=q.device) if keep_parts else None
     lse = th.empty((n, 2 * h), dtype=_lse_dtype(q), device=q.device)
-    _terms_call("attention_diff_forward", graph, elem, _capi.TERMS_DIFF_FWD, e, max(n, k.size(0)), h, d, nb, q.device,
+    _terms_call("attention_diff_forward", graph, elem, _capi.TERMS_DIFF_FWD, e, (n, k.size(0)), h, d, nb, q.device,
                 [_p(q), _p(k), _p(v), _p(lam), _p(bucket), _p(table), nb, float(scale), _p(o), _p(parts), _p(lse)]
                 + ([] if graph[0] is None else [e]) + [n, k.size(0), h, d])
     return o, lse, parts
@@ -996,7 +999,7 @@ def _diff_backward(graph, e, q, k, v, lam, parts, lse, d_o, scale, bucket, table
     if parts.shape != (n, h, 2, 2 * d) or parts.dtype != _lse_dtype(q) or d_o.shape != (n, h, 2 * d) or lse.shape != (n, 2 * h) or lse.dtype != _lse_dtype(q):
         raise RuntimeError("parts, lse and d_o must have the forward's shapes and types")
     out = [th.empty_like(t) for t in (q, k, v, lam)] + ([th.empty_like(table)] if nb else [])
-    _terms_call("attention_diff_backward", graph, elem, _capi.TERMS_DIFF_BWD, e, max(n, k.size(0)), h, d, nb, q.device,
+    _terms_call("attention_diff_backward", graph, elem, _capi.TERMS_DIFF_BWD, e, (n, k.size(0)), h, d, nb, q.device,
                 [_p(q), _p(k), _p(v), _p(lam), _p(bucket), _p(table), nb, _p(parts), _p(lse), _p(d_o), float(scale)]
                 + [_p(t) for t in out] + ([] if nb else [None]) + ([] if graph[0] is None else [e]) + [n, k.size(0), h, d])
     return out

@@ -42,6 +42,17 @@ enum {
 /* Bytes of workspace of one call.  n_nodes: the larger of n_dst and n_src; H, D, n_buckets as in the call. */
 size_t graphop_terms_workspace_bytes(int op, int64_t n_edges, int64_t n_nodes, int H, int D, int n_buckets, int elem_bytes,
                                      int index_bytes);
+/*
+ * The same of one call on plans (plan_t: a backward's second one, else null).  Calls on a dense band run on the tensor cores where all of this
+ * holds: bf16; 64 features of v a head; at most 255 buckets; no more node rows than the plan has nodes; a mean of at least a neighbour
+ * per 16 columns of its span, rounded up to 64, in the plan, or in both plans of a backward; sums 32-byte aligned; a workspace of this
+ * size.  It is more than the size above where a narrow band's tiles need it, for bucket ids and three bytes of score gradient per tile
+ * element, head and map; with that size alone, and in every other case, a call runs the same kernels as on chunk tables.
+ * On the tensor cores probabilities and score gradients are rounded to bf16 before the products with v, k, q and d_o (the
+ * forward of two maps adds what that leaves off), in the other kernels they are not.
+ */
+size_t graphop_terms_workspace_bytes_planned(int op, const graphop_plan_t* plan_r, const graphop_plan_t* plan_t, int64_t n_dst,
+                                             int64_t n_src, int H, int D, int n_buckets, int elem_bytes);
 
 #define GRAPHOP_DECLARE_TERMS(SUF, CT, I)                                                                                            \
   int graphop_attention_bucket_forward_##SUF(const I* row, const I* indptr, const I* indices, int64_t n_chunks, const CT* q,         \

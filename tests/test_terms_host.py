@@ -1,4 +1,5 @@
 """Attention layers with learned score terms, more of what needs no GPU."""
+import ctypes
 import math
 import os
 import subprocess
@@ -7,7 +8,7 @@ import pytest
 import torch as th
 
 from helpers import ROOT, random_graph
-from custom_op_benchmark_b200 import build
+from custom_op_benchmark_b200 import _capi, build
 from oracle import terms_f64 as ref
 
 
@@ -41,3 +42,37 @@ def test_every_shape_fits_the_workspace_it_asks_for(tmp_path):
     assert res.returncode == 0, res.stderr
     res = subprocess.run([str(exe)], capture_output=True, text=True)
     assert res.returncode == 0, res.stdout
+
+
+def _band_plan(n, degree, span):
+    """What the size functions read of a plan: numbers, and pointers that are there."""
+    return _capi.Plan(n_chunks=n, n_edges=n * degree, n_nodes=n, node_lo=4096, node_deg=4096, node_first=4096, tile_lo=4096,
+                      flags=_capi.PLAN_DENSE_BAND, band_span=span)
+
+
+@pytest.mark.parametrize("n", [300, 4096, 40000, 200000])
+@pytest.mark.parametrize("h", [1, 8])
+@pytest.mark.parametrize("op,buckets", [(_capi.TERMS_BUCKET_BWD, 32), (_capi.TERMS_DIFF_BWD, 32), (_capi.TERMS_BUCKET_FWD, 32),
+                                        (_capi.TERMS_DIFF_FWD, 0)])
+def test_a_plan_that_the_tiles_serve_asks_for_their_room(n, h, op, buckets):
+    lib = _capi.lib()
+    diff, backward = op in (_capi.TERMS_DIFF_FWD, _capi.TERMS_DIFF_BWD), op in (_capi.TERMS_BUCKET_BWD, _capi.TERMS_DIFF_BWD)
+    d, columns = (32, 2 * h) if diff else (64, h)
+
+    def sizes(degree, span, elem=2, d=d, buckets=buckets, rows=n, second=True):
+        plan = _band_plan(n, degree, span)
+        other = ctypes.byref(plan) if backward and second else None
+        return (lib.graphop_terms_workspace_bytes_planned(op, ctypes.byref(plan), other, rows, rows, h, d, buckets, elem),
+                lib.graphop_terms_workspace_bytes(op, n * degree, rows, h, d, buckets, elem, 4))
+    # window 8: 17 neighbours, 192 columns
+    planned, plain = sizes(17, 144)
+    assert planned >= plain
+    if buckets:
+        per_element = 2 + 3 * columns if backward else 1         # ids of both sides, score gradients
+        assert planned >= (n // 128) * 128 * 192 * per_element
+    for other in (sizes(11, 144), sizes(17, 144, elem=4), sizes(17, 144, d=2 * d), sizes(17, 144, rows=n + 1), sizes(17, 385),
+                  sizes(17, 144, buckets=256)):
+        assert other[0] == other[1] > 0
+    if backward:
+        assert sizes(17, 144, second=False)[0] == 0
+    assert lib.graphop_terms_workspace_bytes_planned(op, None, None, n, n, h, d, buckets, 2) == 0
