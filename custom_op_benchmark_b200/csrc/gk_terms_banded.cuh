@@ -30,7 +30,7 @@ struct TermsTile {
   int pitch;                                 // columns of the band per tile, a multiple of 64
   int buckets;
   const int32_t *node_lo, *node_deg;         // of the owning side
-  int* dirty;                                // (H, tiles)
+  int* dirty;                                // (H, tiles): 0, kTileAgain or kTileLost
   long long n_own, n_other;
   int H;
   float scale;
@@ -444,7 +444,7 @@ terms_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   bad = __syncthreads_or(bad);
-  if (tid == 0) p.dirty[(size_t)head * gridDim.x + blockIdx.x] = bad;
+  if (tid == 0) p.dirty[(size_t)head * gridDim.x + blockIdx.x] = bad ? kTileAgain : 0;
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmem) : "memory");
 }
@@ -730,7 +730,7 @@ __device__ __forceinline__ void terms_backward_tile(const CUtensorMap& map_a, co
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   bad = __syncthreads_or(bad);
-  if (tid == 0) p.dirty[(size_t)head * tiles + blockIdx.x] = bad;
+  if (tid == 0) p.dirty[(size_t)head * tiles + blockIdx.x] = !ok ? kTileLost : bad ? kTileAgain : 0;
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmem) : "memory");
 }
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
     *reinterpret_cast<__nv_bfloat162*>(x + at * kD + 2 * lane) = __floats2bfloat162_rn(u, v);
   };
   for (int f = blockIdx.x * 8 + (threadIdx.x >> 5); f < total; f += warps) {
-    if (!t.dirty[f]) continue;
+    if (t.dirty[f] != kTileAgain) continue;
     const int head = f / a.tiles;
     const long long r0 = (long long)(f - head * a.tiles) * kTileM;
     const float lam = kMaps == 2 ? __bfloat162float(t.lam[head]) : 0.f;
@@ -910,81 +910,8 @@ __global__ void __launch_bounds__(256) band_again_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// dT: sums of g by bucket, over the tiles' elements in the threads' order
+// launches
 // ---------------------------------------------------------------------------------------------------------
-// grid: (blocks, H * maps).  A thread takes 8 elements at a time, so that a warp's loads are whole lines, and asks for kAhead such
-// pieces at once; they go into a table of its own, cell b of thread t at b * NT + t: a warp's 32 cells lie in 32 banks.  An element
-// that takes no part has a gradient of zero and goes to one cell more.  Bound by its instructions, about ten per element (with a test
-// per element and the table's stride not known, 14), then by reading the gradients: 6.3M elements of 8 heads 43 us (3.6 TB/s; 28 when
-// the gradients were bfloat16).
-template <int NT>
-__global__ void __launch_bounds__(NT)
-band_bucket_sum_kernel(const unsigned char* __restrict__ ids, const unsigned short* __restrict__ g, const unsigned char* __restrict__ g_low,
-                       long long elements, int buckets, int columns, double* __restrict__ partial) {
-  extern __shared__ float cells[];
-  constexpr int kAhead = 4;
-  const int tid = threadIdx.x, column = blockIdx.y;
-  const long long pieces = elements / 8, stride = (long long)gridDim.x * NT;
-  const uint2* idp = reinterpret_cast<const uint2*>(ids);
-  const uint4* src = reinterpret_cast<const uint4*>(g + (size_t)column * elements);
-  const uint2* src_low = reinterpret_cast<const uint2*>(g_low + (size_t)column * elements);
-  float* mine = cells + tid;
-  for (int b = 0; b <= buckets; ++b) mine[b * NT] = 0.f;
-  const unsigned none = (unsigned)buckets;
-  for (long long i = (long long)blockIdx.x * NT + tid; i < pieces; i += kAhead * stride) {
-    uint2 id[kAhead];
-    uint4 w[kAhead];
-    uint2 l[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) id[k] = i + k * stride < pieces ? __ldg(idp + i + k * stride) : make_uint2(0xffffffffu, 0xffffffffu);
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if ((id[k].x & id[k].y) != 0xffffffffu) {   // else nothing takes part, and nothing was stored
-        w[k] = __ldg(src + i + k * stride);
-        l[k] = __ldg(src_low + i + k * stride);
-      }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if ((id[k].x & id[k].y) == 0xffffffffu) continue;
-      const unsigned v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const unsigned b = min(((j < 4 ? id[k].x : id[k].y) >> (8 * (j & 3))) & 255u, none);
-        // bytes of the float, from the highest: two of the upper plane, one of the lower, zero
-        const unsigned high = (j & 1) ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16, next = j < 4 ? l[k].x : l[k].y;
-        mine[b * NT] += __uint_as_float(__byte_perm(high, next, 0x3200 | ((4 + (j & 3)) << 4)));
-      }
-    }
-  }
-  __syncthreads();
-  const int warp = tid >> 5, lane = tid & 31;
-  for (int b = warp; b < buckets; b += NT / 32) {   // a bucket per warp: the threads' cells in order, by halves
-    double s = 0;
-#pragma unroll
-    for (int t = 0; t < NT; t += 32) s += (double)cells[b * NT + t + lane];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
-    if (lane == 0) partial[((size_t)blockIdx.x * buckets + b) * columns + column] = s;
-  }
-}
-inline int run_band_bucket_sum(const BandSumShape& s, const unsigned char* ids, const unsigned short* g, const unsigned char* g_low,
-                               long long elements, int buckets, int columns, double* partial, __nv_bfloat16* out, cudaStream_t st) {
-  const auto launch = [&](auto kernel, std::atomic<bool> (&configured)[64]) -> int {
-    GK_TRY(allow_smem(kernel, 56 * 1024, configured));
-    kernel<<<dim3((unsigned)s.blocks, (unsigned)columns), s.threads, s.smem, st>>>(ids, g, g_low, elements, buckets, columns, partial);
-    GK_LAUNCHED("band_bucket_sum");
-    return GRAPHOP_OK;
-  };
-  static std::atomic<bool> c128[64], c64[64], c32[64];
-  if (s.threads == 128) GK_TRY(launch(band_bucket_sum_kernel<128>, c128));
-  else if (s.threads == 64) GK_TRY(launch(band_bucket_sum_kernel<64>, c64));
-  else GK_TRY(launch(band_bucket_sum_kernel<32>, c32));
-  const int cells = buckets * columns;
-  bucket_total_kernel<__nv_bfloat16><<<(cells + 7) / 8, 256, 0, st>>>(partial, s.blocks, cells, 1.0, out);
-  GK_LAUNCHED("bucket_total");
-  return GRAPHOP_OK;
-}
-
 inline BandIds band_ids_of(const graphop_plan_t* plan, const int32_t* eid, long long n, int per, unsigned char* ids) {
   return BandIds{plan->node_lo, plan->node_deg, plan->node_first, plan->tile_lo, eid, n, band_pitch(plan), per, ids};
 }
@@ -1059,7 +986,7 @@ inline int terms_backward(const graphop_plan_t* plan_r, const graphop_plan_t* pl
   GK_LAUNCHED(kMaps == 2 ? "attention_diff_bwd_banded" : "attention_bucket_bwd_banded");
   GK_TRY((run_band_again<1, kMaps, kBucket>(AgainArgs{t, c.q, c.k, c.v, dout, plan_r->node_first, nullptr, c.bucket, (int)tiles}, st)));
   GK_TRY((run_band_again<2, kMaps, kBucket>(AgainArgs{u, c.q, c.k, c.v, dout, plan_t->node_first, plan_t->eid, c.bucket, (int)tiles_t}, st)));
-  if (kBucket) GK_TRY(run_band_bucket_sum(room.sum, room.ids, room.g, room.g_low, room.elements, c.buckets, columns, room.partial, d_table, st));
+  if (kBucket) GK_TRY(run_band_bucket_sum(room, (int)tiles, c.buckets, c.H, kMaps, d_table, st));
   if (kMaps == 2) GK_TRY((run_bucket_sum<__nv_bfloat16>(ar, room.t2, c.n_dst, c.H, 1, c.H, nullptr, 1, nullptr, -1.0, d_lam, st)));
   return GRAPHOP_OK;
 }
