@@ -55,7 +55,7 @@ int check_graph(const I* row, const I* indptr, const I* eid, const I* indices, l
 }  // namespace
 }  // namespace gk
 
-extern "C" int graphop_version(void) { return 100; }
+extern "C" int graphop_version(void) { return GRAPHOP_VERSION; }
 
 extern "C" const char* graphop_error_string(int code) {
   switch (code) {

@@ -68,6 +68,12 @@ enum {
   GRAPHOP_OP_ATTENTION_BWD_PAIRS = 10     /* ... with eid_t: room for (p, ds) of every edge and head */
 };
 
+/*
+ * The version of this header, and of the library at run time.  The structs here belong to the version: a library writes the whole of
+ * its own graphop_plan_t, so that a program passes one only where graphop_version() == GRAPHOP_VERSION of the header that it was compiled
+ * with.  101: graphop_plan_t ends with node_first and tile_lo; graphop_terms.h.
+ */
+#define GRAPHOP_VERSION 101
 int graphop_version(void);
 const char* graphop_error_string(int code);
 /* cudaError_t of the most recent failed CUDA call made by this library on this thread. */
@@ -169,6 +175,7 @@ enum {
 };
 #define GRAPHOP_BAND_MAX_SPAN 384
 
+/* Its size belongs to GRAPHOP_VERSION: fields are added at the end. */
 typedef struct graphop_plan {
   int64_t n_chunks;        /* chunks of the table the plan was built from */
   int64_t n_edges;         /* CSR positions */

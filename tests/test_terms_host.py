@@ -76,3 +76,16 @@ def test_a_plan_that_the_tiles_serve_asks_for_their_room(n, h, op, buckets):
     if backward:
         assert sizes(17, 144, second=False)[0] == 0
     assert lib.graphop_terms_workspace_bytes_planned(op, None, None, n, n, h, d, buckets, 2) == 0
+
+
+def test_the_version_belongs_to_the_plan_struct(tmp_path):
+    """A library that writes a longer struct than its caller has says so: when the struct grows, so does the version."""
+    src, exe = tmp_path / "version.c", tmp_path / "version"
+    src.write_text('#include <stdio.h>\n#include "graphop_b200.h"\n'
+                   'int main(void) { printf("%d %d\\n", GRAPHOP_VERSION, (int)sizeof(graphop_plan_t)); return 0; }\n')
+    res = subprocess.run(["gcc", "-std=c99", "-I" + os.path.join(ROOT, "include"), str(src), "-o", str(exe)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    version, size = map(int, subprocess.run([str(exe)], capture_output=True, text=True).stdout.split())
+    assert _capi.lib().graphop_version() == version
+    assert ctypes.sizeof(_capi.Plan) == size
+    assert (version, size) == (101, 112)       # 100: 96
