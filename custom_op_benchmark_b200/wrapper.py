@@ -233,8 +233,8 @@ class GraphAttentionBucket(Function):
 
     @staticmethod
     def forward(ctx, row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, scale):
-        o, lse, sums = _g.attention_bucket_forward(row, indptr, indices, Q, K, V, bucket, table, scale, keep_sums=True)
-        ctx.save_for_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, sums, lse)
+        o, lse, *sums = _g.attention_bucket_forward(row, indptr, indices, Q, K, V, bucket, table, scale, keep_sums=any(ctx.needs_input_grad))
+        ctx.save_for_backward(row, indptr, indices, col, indptr_t, eid_t, indices_t, Q, K, V, bucket, table, sums[0] if sums else None, lse)
         ctx.scale = scale
         return o
 
@@ -260,8 +260,8 @@ class GraphAttentionBucketPlanned(Function):
     @staticmethod
     def forward(ctx, plan_r, plan_t, Q, K, V, bucket, table, scale):
         _g.check_plan_rows(plan_r, plan_t, Q.size(0), K.size(0))
-        o, lse, sums = _g.attention_bucket_forward_planned(plan_r, Q, K, V, bucket, table, scale, keep_sums=True)
-        ctx.save_for_backward(Q, K, V, bucket, table, sums, lse)
+        o, lse, *sums = _g.attention_bucket_forward_planned(plan_r, Q, K, V, bucket, table, scale, keep_sums=any(ctx.needs_input_grad))
+        ctx.save_for_backward(Q, K, V, bucket, table, sums[0] if sums else None, lse)
         ctx.plans, ctx.scale = (plan_r, plan_t), scale
         return o
 

@@ -8,7 +8,7 @@ import pytest
 import torch as th
 
 from helpers import ROOT, random_graph
-from custom_op_benchmark_b200 import _capi, build
+from custom_op_benchmark_b200 import _capi, build, graphop, wrapper
 from oracle import terms_f64 as ref
 
 
@@ -89,3 +89,33 @@ def test_the_version_belongs_to_the_plan_struct(tmp_path):
     assert _capi.lib().graphop_version() == version
     assert ctypes.sizeof(_capi.Plan) == size
     assert (version, size) == (101, 112)       # 100: 96
+
+
+class _Context:
+    """What torch.autograd.Function hands a forward."""
+
+    def __init__(self, needs):
+        self.needs_input_grad = needs
+
+    def save_for_backward(self, *tensors):
+        self.saved = tensors
+
+
+@pytest.mark.parametrize("planned", [False, True])
+@pytest.mark.parametrize("wanted", [False, True])
+def test_the_unrounded_sums_are_kept_where_a_gradient_is_asked_for(monkeypatch, planned, wanted):
+    """The Functions without the compiled nodes: the bias layer's sums are a tensor of float32 as large as q."""
+    name, seen, t = "attention_bucket_forward" + ("_planned" if planned else ""), [], th.zeros(2, 1, 16)
+
+    def forward(*args, keep_sums):
+        seen.append(keep_sums)
+        return (t, t, t) if keep_sums else (t, t)
+    monkeypatch.setattr(graphop, name, forward)
+    if planned:
+        monkeypatch.setattr(graphop, "check_plan_rows", lambda *a: None)
+    function, n_graph = (wrapper.GraphAttentionBucketPlanned, 2) if planned else (wrapper.GraphAttentionBucket, 7)
+    needs = [False] * (n_graph + 6)
+    needs[n_graph + 4] = wanted                 # the table
+    ctx = _Context(tuple(needs))
+    assert function.forward(ctx, *[None] * n_graph, t, t, t, None, t, 1.0) is t
+    assert seen == [wanted] and (ctx.saved[-2] is t) == wanted
