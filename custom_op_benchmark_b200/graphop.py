@@ -707,7 +707,7 @@ def attention_backward_planned(plan_r, plan_t, q, k, v, o, lse, d_o, scale):
 # ------------------------------------------------------------------------------------------
 def bucket_limits(num_buckets, max_distance):
     """The distances at which the buckets of one direction begin, but for the first: bucket b holds the distances that
-    at least b of them do not exceed.  The first half of the buckets hold one distance each; the others share what lies
+    exactly b of them do not exceed.  The first half of the buckets hold one distance each; the others share what lies
     between there and ``max_distance`` evenly over its logarithm, and the last one also holds everything farther:
     bucket(x) = half + floor((num_buckets - half) * ln(x / half) / ln(max_distance / half)).  In whole numbers: a limit is
     the smallest x with x^m * half^t >= max_distance^t * half^m, m = num_buckets - half, t = bucket - half."""

@@ -119,3 +119,13 @@ def test_the_unrounded_sums_are_kept_where_a_gradient_is_asked_for(monkeypatch, 
     ctx = _Context(tuple(needs))
     assert function.forward(ctx, *[None] * n_graph, t, t, t, None, t, 1.0) is t
     assert seen == [wanted] and (ctx.saved[-2] is t) == wanted
+
+
+def test_a_bucket_holds_the_distances_that_exactly_so_many_limits_do_not_exceed():
+    """As the docstring says: the buckets do not overlap, and the reference puts every distance into the same one."""
+    assert "exactly b of them" in graphop.bucket_limits.__doc__
+    at = graphop.bucket_limits(10, 300)
+    x = th.arange(400)
+    want = ref.relative_buckets(th.zeros(400, dtype=th.int64), x, 10, 300, False, th.zeros(1, dtype=th.int64), -x)
+    for b in range(10):
+        assert ((want == b) == (th.tensor([sum(a <= d for a in at) for d in x.tolist()]) == b)).all()
