@@ -715,6 +715,8 @@ def bucket_limits(num_buckets, max_distance):
     half = num_buckets // 2
     if num_buckets < 2 or max_distance <= half:
         raise ValueError("relative positions need two buckets or more a direction, and a max_distance beyond the exact ones")
+    if max_distance >= 2 ** 63:
+        raise ValueError("max_distance must be a distance of 64-bit positions")
     m, found = num_buckets - half, list(range(1, half + 1))
     for t in range(1, m):
         want = max_distance ** t * half ** m
@@ -731,7 +733,10 @@ def _limits(num_buckets, max_distance, bidirectional):
     """The limits of a direction as the library takes them, packed once: a conversion of hundreds of them costs more than the call."""
     if bidirectional and num_buckets % 2:
         raise ValueError("num_buckets must be even for both directions")
-    return _limits_of(int(num_buckets) // 2 if bidirectional else int(num_buckets), int(max_distance))
+    num_buckets = int(num_buckets) // 2 if bidirectional else int(num_buckets)
+    if num_buckets > 1024:
+        raise ValueError("relative positions take at most 1024 buckets a direction")
+    return _limits_of(num_buckets, int(max_distance))
 
 
 @functools.lru_cache(maxsize=64)
@@ -762,7 +767,7 @@ def relative_buckets(row, indptr, indices, num_buckets, max_distance, bidirectio
     ``bidirectional``: half of the buckets are for positions ahead (a positive difference), the others for the rest;
     without it all are for positions behind, and those ahead share bucket 0.  Within a direction the distances are
     shared out as ``bucket_limits`` says.  ``dst_pos`` and ``src_pos`` (index type) default to the node ids; every
-    node that an edge names needs a position."""
+    node that an edge names needs a position.  At most 1024 buckets a direction, a ``max_distance`` below 2^63."""
     limits = _limits(num_buckets, max_distance, bidirectional)
     native = native_functions_if_built()
     if native is not None:

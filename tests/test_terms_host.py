@@ -129,3 +129,19 @@ def test_a_bucket_holds_the_distances_that_exactly_so_many_limits_do_not_exceed(
     want = ref.relative_buckets(th.zeros(400, dtype=th.int64), x, 10, 300, False, th.zeros(1, dtype=th.int64), -x)
     for b in range(10):
         assert ((want == b) == (th.tensor([sum(a <= d for a in at) for d in x.tolist()]) == b)).all()
+
+
+@pytest.mark.parametrize("count,reach,both,match", [(32, 2 ** 63, False, "64-bit"), (32, 10 ** 400, True, "64-bit"),
+                                                    (1025, 10 ** 6, False, "1024"), (2050, 10 ** 6, True, "1024"), (10 ** 6, 10 ** 9, True, "1024")])
+def test_buckets_beyond_what_the_library_takes_are_refused_as_such(count, reach, both, match):
+    """Not as an overflow of the packing, and before a limit is computed; nothing of the graph is looked at."""
+    with pytest.raises(ValueError, match=match):
+        graphop.relative_buckets(None, None, None, count, reach, both)
+    with pytest.raises(ValueError, match=match):
+        graphop.relative_buckets_planned(None, count, reach, both)
+
+
+def test_the_largest_limits_fit_their_packing():
+    at = graphop.bucket_limits(1024, 2 ** 63 - 1)
+    assert len(at) == 1023 and at == sorted(at) and at[-1] < 2 ** 63
+    assert len(graphop._limits(2048, 2 ** 63 - 1, True)) == 1023 * 8
