@@ -960,7 +960,10 @@ def attention_bucket_backward(row, indptr, indices, col, indptr_t, eid_t, indice
 
 
 def attention_bucket_forward_planned(plan, q, k, v, bucket, table, scale, keep_sums=False):
-    """attention_bucket_forward on a plan of the row CSR."""
+    """attention_bucket_forward on a plan of the row CSR.  On a dense band of bfloat16 with 64 features a head, up to 255 buckets and a
+    mean of a neighbour per 16 columns of its span it runs on the tensor cores, here and in the backward: probabilities and score gradients
+    are rounded to bfloat16 before the products, which the chunk-table call does not do.  Every other plan gives the chunk-table
+    call's bits."""
     native = native_functions_if_built()
     if native is not None:
         out = native.attention_bucket_forward_planned(plan.native(), q, k, v, bucket, table, scale, keep_sums)
@@ -1031,7 +1034,8 @@ def attention_diff_backward(row, indptr, indices, col, indptr_t, eid_t, indices_
 
 
 def attention_diff_forward_planned(plan, q, k, v, lam, scale, bucket=None, table=None, keep_parts=True):
-    """attention_diff_forward on a plan of the row CSR."""
+    """attention_diff_forward on a plan of the row CSR; on a dense band, with 64 features of v a head, as
+    attention_bucket_forward_planned (probabilities of the forward are not rounded here: a second product adds what is left)."""
     native = native_functions_if_built()
     if native is not None:
         return native.attention_diff_forward_planned(plan.native(), q, k, v, lam, scale, bucket, table, keep_parts)
