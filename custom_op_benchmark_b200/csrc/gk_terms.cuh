@@ -900,7 +900,7 @@ inline int terms_backward(const GS& gs_r, const GS& gs_c, bool has_eid_t, long l
   return run_terms_src<T>(ar, g, c, dout, pd, Hp, dk, dv, st);
 }
 
-// bytes of workspace of either direction
+// bytes of workspace of either direction, by the walkers
 inline size_t terms_bytes(bool diff, bool backward, long long E, long long n_nodes, int H, int D, int buckets, int elem, int index_bytes) {
   const size_t acc = elem == 8 ? 8 : 4;
   const int maps = diff ? 2 : 1, columns = H * maps, row_d = D * maps;

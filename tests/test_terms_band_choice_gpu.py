@@ -1,6 +1,7 @@
 """Which kernels a call on a dense-band plan runs (tensor cores where a node has enough neighbours for the columns that a tile computes,
 else the walkers), that either answer is right, and bands whose two sides have different numbers of tiles."""
 import ctypes
+import threading
 
 import pytest
 import torch as th
@@ -104,3 +105,26 @@ def test_without_the_plans_workspace_the_walkers_run(diff, buckets):
         layer.check([o] + out, STAGED if tiles else 0.0)
     assert getattr(lib, name)(plans[0].ref(), plans[1].ref(), *args, *[p(t) for t in out], n, n, h, d, p(ws), 4096,
                               th.cuda.current_stream().cuda_stream) == _capi.ERR_WORKSPACE
+
+
+def test_bands_on_several_threads_and_streams():
+    """Blocks of different kernels share the SMs' tensor memory and shared memory; everyone gets the bits of a call alone."""
+    layers = [_layer(graphs.banded_graph(2, 700, w), diff, buckets, 4, 54) for w, (diff, buckets) in zip((64, 30, 128), KINDS)]
+    plans = [layer.plans() for layer in layers]
+    want = [layer.step(p) for layer, p in zip(layers, plans)]
+    wrong = []
+
+    def work(i):
+        with th.cuda.stream(th.cuda.Stream()):
+            for _ in range(10):
+                got = layers[i].step(plans[i])
+                th.cuda.current_stream().synchronize()
+                if not all(th.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    th.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i % 3,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
